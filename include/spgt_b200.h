@@ -32,6 +32,11 @@ extern "C" {
 #define SPGT_ACT_SILU 2
 #define SPGT_ACT_SILU2 3          /* SiLU applied twice, as the reference's UpScaler2D does */
 
+/* Element types of the training operators at the end of this file. */
+#define SPGT_F32 0
+#define SPGT_BF16 1
+#define SPGT_F16 2
+
 typedef void* spgt_stream_t;
 
 /* Human-readable text for an SPGT_ERR_* code; never NULL. */
@@ -409,6 +414,41 @@ int spgt_darcy_forward(const spgt_darcy_model* model, const float* node, const f
 /* The same with the head's second bias read from device memory (head_b2 [1], NULL: model->b2): no copy to the host for a new model. */
 int spgt_darcy_forward_devbias(const spgt_darcy_model* model, const float* head_b2, const float* node, const float* position, const float* grid,
                                float* out, int B, float* const* taps, void* workspace, size_t workspace_bytes, spgt_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Training operators without a counterpart in the reference: activation checkpoints in 8 bits, and group
+ * normalisation, channels last.  `dtype` is the type of x, y, dx, dy; parameters, statistics and their gradients are fp32.
+ *
+ * A checkpoint of n values, in row-major order, is codes [n] and steps [ceil(n / 32)]: value i is codes[i] * 2^(steps[i / 32] - 127).
+ * The step of 32 consecutive values is the smallest power of two (2^-126 at least) of which the largest magnitude among them is
+ * less than 127.5; codes are rounded to nearest even, so a value is off by half a step at most.  A NaN or an infinity makes
+ * all 32 values NaN (step 255).  Magnitudes beyond 63.5 * 2^122 become 63 * 2^122 (64 would be an infinity).
+ * ------------------------------------------------------------------------------------------- */
+
+/* codes, steps = checkpoint of x [n]; with y, also y = act(x).  y may be x. */
+int spgt_compress8(const void* x, int dtype, int act, void* y, int8_t* codes, uint8_t* steps, int64_t n, spgt_stream_t stream);
+/* out [n] = the checkpoint's values v, or with dy [n]: dy * act'(v).  out may be dy.  fp16: values beyond 65504 become 65504. */
+int spgt_restore8(const int8_t* codes, const uint8_t* steps, const void* dy, int act, void* out, int dtype, int64_t n, spgt_stream_t stream);
+
+/* dw [N, K] = dy^T v and, unless NULL, db [N] = column sums of dy, for dy [rows, N] and a checkpoint of v [rows, K].
+ * 0 bytes: unsupported sizes. */
+size_t spgt_weight_gradient8_workspace_bytes(int N, int K, int64_t rows);
+int spgt_weight_gradient8(const void* dy, int dtype, const int8_t* codes, const uint8_t* steps, float* dw, float* db, int N, int K,
+                          int64_t rows, void* workspace, size_t workspace_bytes, spgt_stream_t stream);
+
+/* y = act((x - m) / sqrt(v + eps) * w + b) for x, y [N, P, C] with mean m and biased variance v of each sample's and group's P * C / G
+ * values; w, b [C] or NULL (1, 0).  stats [N, G, 2] receives m and 1 / sqrt(v + eps).  With codes and steps a checkpoint of x is
+ * written as well.  G divides C; C is up to 512, or up to 2048 (fp32) and 4096 (bf16, fp16) in multiples of 16 bytes.
+ * 0 bytes: unsupported sizes.  y may be x unless a checkpoint is written. */
+size_t spgt_group_norm_workspace_bytes(int N, int64_t P, int C, int G, int dtype);
+int spgt_group_norm_fwd(const void* x, const float* w, const float* b, void* y, float* stats, int8_t* codes, uint8_t* steps,
+                        int N, int64_t P, int C, int G, float eps, int act, int dtype, void* workspace, size_t workspace_bytes,
+                        spgt_stream_t stream);
+/* dx [N, P, C], dw [C], db [C] (dw, db may be NULL) for dy, the forward's stats, and x or a checkpoint of it (codes not NULL). */
+size_t spgt_group_norm_bwd_workspace_bytes(int N, int64_t P, int C, int G, int dtype);
+int spgt_group_norm_bwd(const void* dy, const void* x, const int8_t* codes, const uint8_t* steps, const float* w, const float* b,
+                        const float* stats, void* dx, float* dw, float* db, int N, int64_t P, int C, int G, int act, int dtype,
+                        void* workspace, size_t workspace_bytes, spgt_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -109,6 +109,14 @@ SIGNATURES = {
     'spgt_darcy_launches': (_i, [_f, _i]),
     'spgt_darcy_forward': (_i, [_f] * 5 + [_i, _f, _f, _sz, _st]),
     'spgt_darcy_forward_devbias': (_i, [_f] * 6 + [_i, _f, _f, _sz, _st]),
+    'spgt_compress8': (_i, [_f, _i, _i, _f, _f, _f, C.c_int64, _st]),
+    'spgt_restore8': (_i, [_f, _f, _f, _i, _f, _i, C.c_int64, _st]),
+    'spgt_weight_gradient8_workspace_bytes': (_sz, [_i, _i, C.c_int64]),
+    'spgt_weight_gradient8': (_i, [_f, _i, _f, _f, _f, _f, _i, _i, C.c_int64, _f, _sz, _st]),
+    'spgt_group_norm_workspace_bytes': (_sz, [_i, C.c_int64, _i, _i, _i]),
+    'spgt_group_norm_fwd': (_i, [_f] * 7 + [_i, C.c_int64, _i, _i, _fl, _i, _i, _f, _sz, _st]),
+    'spgt_group_norm_bwd_workspace_bytes': (_sz, [_i, C.c_int64, _i, _i, _i]),
+    'spgt_group_norm_bwd': (_i, [_f] * 10 + [_i, C.c_int64, _i, _i, _i, _i, _f, _sz, _st]),
     'spgt_spectral_conv2d_fwd': (_i, [_f, _f, _f, _f, _f, _f, _f, _sz, _f, _i, _i, _i, _i, _i, _st]),
 }
 

@@ -782,3 +782,188 @@ def darcy_forward(plan: DarcyPlan, node: Tensor, position: Tensor, grid: Tensor,
         _call('spgt_darcy_forward_devbias', plan.address, plan.head_b2, node.data_ptr(), position.data_ptr(), grid.data_ptr(), out.data_ptr(), B, want,
               workspace.data_ptr(), need, _stream(), kernels=kernels)
     return out
+
+
+# ---------------------------------------------------------------------------------------------------------
+# activation checkpoints in 8 bits, and group normalisation, for training
+# ---------------------------------------------------------------------------------------------------------
+DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype(t: Tensor, name: str) -> int:
+    if not isinstance(t, Tensor):
+        raise TypeError(f'{name} must be a torch.Tensor')
+    if t.dtype not in DTYPE:
+        raise TypeError(f'{name} must be float32, bfloat16 or float16, got {t.dtype}')
+    _chk(t, name, t.dtype)
+    return DTYPE[t.dtype]
+
+
+def _aligned(t: Tensor) -> Tensor:
+    """t where 16-byte accesses may start: a copy of a view that begins elsewhere."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class Checkpoint8:
+    """A tensor kept in 8 bits: codes [n] (int8) and steps [ceil(n / 32)] (uint8), value i = codes[i] * 2^(steps[i // 32] - 127) in
+    row-major order; off by half a step at most, and a step is less than 1/63 of the largest magnitude among its 32 values.
+    Not finite values make their 32 values NaN."""
+    __slots__ = ('codes', 'steps', 'shape', 'dtype')
+
+    def __init__(self, codes: Tensor, steps: Tensor, shape: Sequence[int], dtype=torch.float32):
+        _chk(codes, 'codes', torch.int8); _chk(steps, 'steps', torch.uint8)
+        n = math.prod(shape)
+        if codes.numel() != n or steps.numel() != (n + 31) // 32:
+            raise ValueError(f'a checkpoint of {tuple(shape)} has {n} codes and {(n + 31) // 32} steps')
+        if codes.device != steps.device:
+            raise ValueError('codes and steps must be on the same device')
+        if dtype not in DTYPE:
+            raise TypeError(f'dtype must be float32, bfloat16 or float16, got {dtype}')
+        self.codes, self.steps, self.shape, self.dtype = _aligned(codes), steps, torch.Size(shape), dtype
+
+    @classmethod
+    def _empty(cls, x: Tensor):
+        self, n = cls.__new__(cls), x.numel()
+        self.shape, self.dtype = x.shape, x.dtype
+        self.codes = torch.empty(n, dtype=torch.int8, device=x.device)
+        self.steps = torch.empty((n + 31) // 32, dtype=torch.uint8, device=x.device)
+        return self
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.steps.numel()
+
+    def restore(self) -> Tensor:
+        return restore8(self)
+
+
+def _same(t: Tensor, name: str, shape, device) -> Tensor:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{name} must be {tuple(shape)}, got {tuple(t.shape)}')
+    if t.device != device:
+        raise ValueError(f'{name} must be on {device}, got {t.device}')
+    return t
+
+
+def compress8(x: Tensor) -> Checkpoint8:
+    """x in 8 bits."""
+    code = _dtype(x, 'x')
+    x = _aligned(x)
+    with _device(x.device):
+        kept = Checkpoint8._empty(x)
+        _call('spgt_compress8', x.data_ptr(), code, 0, None, kept.codes.data_ptr(), kept.steps.data_ptr(), x.numel(), _stream())
+    return kept
+
+
+def restore8(kept: Checkpoint8) -> Tensor:
+    """The values of a checkpoint, in the type of the tensor it was made from."""
+    with _device(kept.device):
+        out = torch.empty(kept.shape, dtype=kept.dtype, device=kept.device)
+        _call('spgt_restore8', kept.codes.data_ptr(), kept.steps.data_ptr(), None, 0, out.data_ptr(), DTYPE[kept.dtype], out.numel(), _stream())
+    return out
+
+
+def activation8(x: Tensor, act) -> Tuple[Tensor, Checkpoint8]:
+    """(act(x), x in 8 bits) in one pass."""
+    code = _dtype(x, 'x')
+    x = _aligned(x)
+    with _device(x.device):
+        kept, y = Checkpoint8._empty(x), torch.empty_like(x)
+        _call('spgt_compress8', x.data_ptr(), code, act_code(act), y.data_ptr(), kept.codes.data_ptr(), kept.steps.data_ptr(), x.numel(), _stream())
+    return y, kept
+
+
+def activation8_backward(grad_out: Tensor, kept: Checkpoint8, act) -> Tensor:
+    """grad_out * act'(kept)."""
+    code = _dtype(grad_out, 'grad_out')
+    _same(grad_out, 'grad_out', kept.shape, kept.device)
+    grad_out = _aligned(grad_out)
+    with _device(kept.device):
+        dx = torch.empty_like(grad_out)
+        _call('spgt_restore8', kept.codes.data_ptr(), kept.steps.data_ptr(), grad_out.data_ptr(), act_code(act), dx.data_ptr(), code, dx.numel(), _stream())
+    return dx
+
+
+def weight_gradient8(grad_out: Tensor, kept: Checkpoint8, column_sums: bool = True):
+    """(grad_out^T kept [N, K], column sums of grad_out [N] or None), fp32, for grad_out [..., N] and a checkpoint of [..., K]: weight and
+    bias gradient of a linear layer from its input in 8 bits."""
+    code = _dtype(grad_out, 'grad_out')
+    if grad_out.dim() < 1 or len(kept.shape) != grad_out.dim() or grad_out.shape[:-1] != kept.shape[:-1]:
+        raise ValueError('grad_out must be [..., N] for a checkpoint of [..., K]')
+    if grad_out.device != kept.device:
+        raise ValueError('grad_out and the checkpoint must be on the same device')
+    grad_out = _aligned(grad_out)
+    N, K, rows = grad_out.shape[-1], kept.shape[-1], math.prod(kept.shape[:-1])
+    need = int(lib.spgt_weight_gradient8_workspace_bytes(N, K, rows))
+    if need == 0:
+        raise ValueError(f'unsupported sizes N={N}, K={K}, rows={rows}')
+    with _device(kept.device):
+        dw = torch.empty(N, K, dtype=torch.float32, device=kept.device)
+        db = torch.empty(N, dtype=torch.float32, device=kept.device) if column_sums else None
+        ws = torch.empty(need, dtype=torch.uint8, device=kept.device)
+        _call('spgt_weight_gradient8', grad_out.data_ptr(), code, kept.codes.data_ptr(), kept.steps.data_ptr(), dw.data_ptr(), _p(db), N, K, rows,
+              ws.data_ptr(), need, _stream(), kernels=2)
+    return dw, db
+
+
+def _norm_sizes(x: Tensor, num_groups: int):
+    if x.dim() < 2:
+        raise ValueError('x must be [N, ..., C]')
+    N, C = x.shape[0], x.shape[-1]
+    if C < 1 or num_groups < 1 or C % num_groups:
+        raise ValueError(f'{C} channels do not divide into {num_groups} groups')
+    return N, math.prod(x.shape[1:-1]), C, num_groups
+
+
+def _norm_param(t: Optional[Tensor], name: str, C: int, device) -> Optional[Tensor]:
+    return None if t is None else _same(_chk(t, name), name, (C,), device)
+
+
+def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1.0e-5, act=None,
+               compress: bool = False):
+    """(act(group_norm(x) * weight + bias), statistics [N, num_groups, 2], x in 8 bits or None) for x [N, ..., C], channels last;
+    weight, bias [C] fp32 or None."""
+    code = _dtype(x, 'x')
+    N, P, C, G = _norm_sizes(x, num_groups)
+    weight, bias = _norm_param(weight, 'weight', C, x.device), _norm_param(bias, 'bias', C, x.device)
+    if not eps >= 0:
+        raise ValueError('eps must not be negative')
+    x = _aligned(x)
+    with _device(x.device):
+        need = int(lib.spgt_group_norm_workspace_bytes(N, P, C, G, code))
+        if need == 0:
+            raise ValueError(f'unsupported number of channels C={C}')
+        y, stats = torch.empty_like(x), torch.empty(N, G, 2, dtype=torch.float32, device=x.device)
+        kept = Checkpoint8._empty(x) if compress else None
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _call('spgt_group_norm_fwd', x.data_ptr(), _p(weight), _p(bias), y.data_ptr(), stats.data_ptr(), kept.codes.data_ptr() if compress else None,
+              kept.steps.data_ptr() if compress else None, N, P, C, G, float(eps), act_code(act), code, ws.data_ptr(), need, _stream(),
+              kernels=0 if x.numel() == 0 else 4 if compress and C % 32 else 3)
+    return y, stats, kept
+
+
+def group_norm_backward(grad_out: Tensor, x, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, act=None):
+    """(dx, dweight [C], dbias [C]) of group_norm for x, the forward's input or a Checkpoint8 of it, and the forward's statistics."""
+    code = _dtype(grad_out, 'grad_out')
+    kept = x if isinstance(x, Checkpoint8) else None
+    if kept is None and _dtype(x, 'x') != code:
+        raise TypeError('x and grad_out must have the same type')
+    N, P, C, G = _norm_sizes(grad_out, num_groups)
+    _same(grad_out, 'grad_out', x.shape, x.device)
+    weight, bias = _norm_param(weight, 'weight', C, x.device), _norm_param(bias, 'bias', C, x.device)
+    _same(_chk(stats, 'stats'), 'stats', (N, G, 2), x.device)
+    grad_out, x, stats = _aligned(grad_out), x if kept is not None else _aligned(x), _aligned(stats)
+    with _device(grad_out.device):
+        need = int(lib.spgt_group_norm_bwd_workspace_bytes(N, P, C, G, code))
+        if need == 0:
+            raise ValueError(f'unsupported number of channels C={C}')
+        dx = torch.empty_like(grad_out)
+        dw, db = (torch.empty(C, dtype=torch.float32, device=dx.device) for _ in range(2))
+        ws = torch.empty(need, dtype=torch.uint8, device=dx.device)
+        _call('spgt_group_norm_bwd', grad_out.data_ptr(), None if kept is not None else x.data_ptr(), kept.codes.data_ptr() if kept is not None else None,
+              kept.steps.data_ptr() if kept is not None else None, _p(weight), _p(bias), stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+              N, P, C, G, act_code(act), code, ws.data_ptr(), need, _stream(), kernels=0 if dx.numel() == 0 else 4)
+    return dx, dw, db
