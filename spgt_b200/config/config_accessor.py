@@ -12,6 +12,7 @@ DARCY_DEFAULTS = dict(
     drop_encoder_attn=0.0, drop_encoder_attn_fc=0.05, dim_encoder_ffn=256, drop_encoder_ffn=0.05, acti_encoder_ffn='relu',
     num_decoder_layer=2, drop_decoder_layer=0.0, acti_decoder_layer='silu', dim_spatial_hidden=32, num_frequence_mode=12,
     seed=1127802, metric_gamma=0.5, lr=1.0e-3, epochs=100, batch_size=4, num_load_worker=8,
+    num_norm_group=0, activation_bits=32,         # not in the reference: group normalisation in the scalers, 8-bit activation checkpoints
 )
 
 

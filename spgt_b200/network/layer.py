@@ -18,7 +18,7 @@ class ParameterWatch:
     """Tells when a module is not as it was seen before: tag() differs after a parameter has been written to (an optimizer step
     bumps the version counters), moved, or replaced, a submodule has been exchanged, or an option that kernels are chosen by
     has been set.  The tree is walked once, not on every call (Module.parameters() takes longer than the launch it would guard)."""
-    OPTIONS = ('activation', 'norm_eps', 'mode', 'structure', 'fused')
+    OPTIONS = ('activation', 'norm_eps', 'mode', 'structure', 'fused', 'num_groups', 'eps')
 
     def __init__(self):
         # one tuple, replaced whole: several threads may share a module.  It holds neither the module nor its __dict__, which would
@@ -137,27 +137,65 @@ def _conv_tc(weight: Tensor, bias: Tensor, cin_pad: int, cout_pad: int, tiles: b
     return ops.TcWeight(w.permute(2, 3, 1, 0).reshape(9 * cin_pad, cout_pad).contiguous()), b
 
 
+class GroupNormAct(torch.nn.Module):
+    """Group normalisation with an activation, channels last: [N, ..., C] in and out.  The reference has no counterpart.
+    activation_bits = 8: training keeps the input in 8 bits."""
+    activation_bits = 32
+
+    def __init__(self, num_groups, num_channels, activation, eps=1.0e-5) -> None:
+        super().__init__()
+        if num_channels % num_groups:
+            raise ValueError(f'{num_channels} channels do not divide into {num_groups} groups')
+        self.num_groups, self.eps, self.activation = num_groups, eps, activation
+        self.weight = torch.nn.Parameter(torch.ones(num_channels))
+        self.bias = torch.nn.Parameter(torch.zeros(num_channels))
+
+    def forward(self, X: Tensor) -> Tensor:
+        from ..extension.bind.normalization import group_norm_act
+        return group_norm_act(X, self.num_groups, self.weight, self.bias, self.eps, self.activation, self.activation_bits)
+
+    def forward_inference(self, X: Tensor, act=None) -> Tensor:
+        """Without gradients; act: an activation in place of the module's own."""
+        return ops.group_norm(X, self.num_groups, self.weight.detach(), self.bias.detach(), self.eps, self.activation if act is None else act)[0]
+
+
 class ConvResBlock2D(_KernelWeights):
     """conv3x3(pad 1) -> [dropout, rate treated as 0] -> activation; NHWC in and out.
-    Reference: network/layer.py:7-24 (NCHW there; the kernels keep channels last throughout)."""
+    Reference: network/layer.py:7-24 (NCHW there; the kernels keep channels last throughout).
+    num_group > 0 puts a group normalisation before the activation, with the largest number of groups up to num_group that divides
+    out_dim."""
 
-    def __init__(self, in_dim, out_dim, kernel_size, padding, droprate, activation) -> None:
+    def __init__(self, in_dim, out_dim, kernel_size, padding, droprate, activation, num_group=0) -> None:
         super().__init__()
         assert kernel_size == 3 and padding == 1
         self.droprate = droprate
         self.activation = activation
         self.conv_layer = torch.nn.Conv2d(in_dim, out_dim, kernel_size=kernel_size, padding=padding)
+        if num_group > 0:
+            self.norm_layer = GroupNormAct(max(g for g in range(1, min(num_group, out_dim) + 1) if out_dim % g == 0), out_dim, activation)
+
+    @property
+    def norm(self):
+        """The block's normalisation, or None."""
+        return self._modules.get('norm_layer')
 
     def kernel_weight(self):
         return self._cached('w', lambda: _conv_kn(self.conv_layer.weight))
 
     def forward_train(self, X: Tensor) -> Tensor:
         """NCHW in and out, differentiable (network/layer.py:16-24 with drop rate 0)."""
-        return _act(self.activation)(self.conv_layer(X))
+        X = self.conv_layer(X)
+        if self.norm is None:
+            return _act(self.activation)(X)
+        return self.norm(X.permute(0, 2, 3, 1).contiguous()).permute(0, 3, 1, 2)
 
     def forward_nhwc(self, X: Tensor, cin_off: int, out: Tensor, cout_off: int, act=None) -> Tensor:
-        """Generic path (any even channel counts / offsets): warp-MMA implicit GEMM."""
+        """Generic path (any even channel counts / offsets): warp-MMA implicit GEMM.  With a normalisation `out` holds its result, and
+        the block's channels are all of `out`."""
         w = self.conv_layer.weight
+        if self.norm is not None:
+            ops.conv3x3(X, cin_off, w.shape[1], self.kernel_weight(), self.conv_layer.bias.detach(), out, cout_off, w.shape[0], None)
+            return out.copy_(self.norm.forward_inference(out, act))
         return ops.conv3x3(X, cin_off, w.shape[1], self.kernel_weight(), self.conv_layer.bias.detach(), out, cout_off,
                            w.shape[0], self.activation if act is None else act)
 
@@ -169,12 +207,23 @@ class ConvResBlock2D(_KernelWeights):
         new tensor [N,H,W,cout_pad] whose channels beyond out_dim hold act(0)."""
         wt, b = self.tc_weight(cin_pad, cout_pad, ops.conv3x3_tiles_pay(*X.shape[:3], X.device))
         out = torch.empty(*X.shape[:3], cout_pad, device=X.device, dtype=X.dtype)
+        if self.norm is not None:
+            cout = self.conv_layer.out_channels
+            Y = self.norm.forward_inference(ops.conv3x3_tc(X, 0, cin_pad, wt, b, out, 0, cout_pad, None)[..., :cout].contiguous(), act)
+            return Y if cout == cout_pad else torch.nn.functional.pad(Y, (0, cout_pad - cout))
         return ops.conv3x3_tc(X, 0, cin_pad, wt, b, out, 0, cout_pad, self.activation if act is None else act)
 
 
 def _act(name):
     """The reference selects SiLU for 'silu' and ReLU for any other string (network/layer.py:14,163)."""
     return torch.nn.functional.silu if name == 'silu' else torch.relu
+
+
+def plain_linears(watch: ParameterWatch, module: torch.nn.Module, *linears) -> bool:
+    """Whether calls of the module's linear layers may be replaced by operators on their parameters: layers of torch's own type that
+    nothing watches, on the GPU."""
+    return (all(type(l) is torch.nn.Linear and l.weight.is_cuda for l in linears)
+            and not watch.observed(module) and not watch.backward_observed(*linears))
 
 
 class FeedForward(_KernelWeights):
@@ -188,6 +237,8 @@ class FeedForward(_KernelWeights):
         self.layer2 = torch.nn.Linear(dim_hidden, out_dim)
         self.fused = True        # one kernel for both GEMMs when the shape is 128 -> 256 -> 128
 
+    activation_bits = 32         # 8: training keeps the inputs of the dense layers and of the activation in 8 bits
+
     def tc_weights(self):
         return self._cached('w1', lambda: _linear_tc(self.layer1.weight)), self._cached('w2', lambda: _linear_tc(self.layer2.weight))
 
@@ -200,4 +251,8 @@ class FeedForward(_KernelWeights):
         return ops.linear_tc(h, w2, self.layer2.bias.detach(), None, residual)
 
     def forward_train(self, X: Tensor) -> Tensor:
+        if self.activation_bits == 8 and plain_linears(self._watch, self, self.layer1, self.layer2):
+            from ..extension.bind.checkpoint8 import activation8, linear8
+            H = activation8(linear8(X, self.layer1.weight, self.layer1.bias), self.activation)
+            return linear8(H, self.layer2.weight, self.layer2.bias)
         return self.layer2(_act(self.activation)(self.layer1(X)))

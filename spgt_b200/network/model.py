@@ -14,7 +14,7 @@ class DownScaler2D(_KernelWeights):
     out_dim-channel full-resolution tensor is never written; conv1..3 write straight into their channel slice
     of the concatenated tensor."""
 
-    def __init__(self, resolution_size, in_dim, out_dim, droprate, activation) -> None:
+    def __init__(self, resolution_size, in_dim, out_dim, droprate, activation, num_group=0) -> None:
         super().__init__()
         assert in_dim == 1, 'the fused first stage handles the single-channel Darcy coefficient'
         self.resolution_size = resolution_size
@@ -23,10 +23,10 @@ class DownScaler2D(_KernelWeights):
         out_dim2 = out_dim // 3
         out_dim3 = int(out_dim - out_dim1 - out_dim2)
         self.dims = (out_dim1, out_dim2, out_dim3)
-        self.conv0 = ConvResBlock2D(in_dim, out_dim, 3, 1, droprate, activation)
-        self.conv1 = ConvResBlock2D(out_dim, out_dim1, 3, 1, droprate, activation)
-        self.conv2 = ConvResBlock2D(out_dim1, out_dim2, 3, 1, droprate, activation)
-        self.conv3 = ConvResBlock2D(out_dim2, out_dim3, 3, 1, droprate, activation)
+        self.conv0 = ConvResBlock2D(in_dim, out_dim, 3, 1, droprate, activation, num_group)
+        self.conv1 = ConvResBlock2D(out_dim, out_dim1, 3, 1, droprate, activation, num_group)
+        self.conv2 = ConvResBlock2D(out_dim1, out_dim2, 3, 1, droprate, activation, num_group)
+        self.conv3 = ConvResBlock2D(out_dim2, out_dim3, 3, 1, droprate, activation, num_group)
 
     def kernel_weight0(self):
         return self._cached('w0', lambda: self.conv0.conv_layer.weight.detach().reshape(-1, 9).t().contiguous())
@@ -34,7 +34,11 @@ class DownScaler2D(_KernelWeights):
     def forward(self, X: Tensor) -> Tensor:
         N, r, _, _ = X.shape
         mid, ra = self.resolution_size[1], self.resolution_size[2]
-        X = ops.conv0_down(X.reshape(N, r, r), self.kernel_weight0(), self.conv0.conv_layer.bias.detach(), mid[0], mid[1], self.activation)
+        X, w, b = X.reshape(N, r, r), self.kernel_weight0(), self.conv0.conv_layer.bias.detach()
+        if self.conv0.norm is None:
+            X = ops.conv0_down(X, w, b, mid[0], mid[1], self.activation)
+        else:                                       # (the statistics need the whole convolution: an interpolation onto its own nodes)
+            X = ops.bilinear(self.conv0.norm.forward_inference(ops.conv0_down(X, w, b, r, r, None)), mid[0], mid[1], self.activation)
         d1, d2, d3 = self.dims
         pad4 = lambda c: (c + 3) // 4 * 4          # the tcgen05 implicit GEMM wants channel counts that are multiples of 4
         X1 = self.conv1.forward_tc(X, X.shape[3], pad4(d1))
@@ -61,12 +65,12 @@ class UpScaler2D(_KernelWeights):
     The activation is applied twice, as in the reference (once inside ConvResBlock2D.forward, network/layer.py:23,
     once more in UpScaler2D.forward, network/model.py:62)."""
 
-    def __init__(self, resolution_size, in_dim, out_dim, droprate, activation) -> None:
+    def __init__(self, resolution_size, in_dim, out_dim, droprate, activation, num_group=0) -> None:
         super().__init__()
         self.resolution_size = resolution_size
         self.droprate = droprate
         self.activation = activation
-        self.conv = ConvResBlock2D(in_dim, out_dim, 3, 1, droprate, activation)
+        self.conv = ConvResBlock2D(in_dim, out_dim, 3, 1, droprate, activation, num_group)
 
     def forward_mid(self, X: Tensor) -> Tensor:
         """Everything up to (not including) the last interpolation: [N, r_mid, r_mid, out_dim]."""

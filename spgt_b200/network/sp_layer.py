@@ -13,10 +13,12 @@ import torch
 from torch import Tensor
 
 from .. import ops
-from .layer import FeedForward, _KernelWeights, _act, _dense, _linear_kn, _linear_tc
+from .layer import FeedForward, _KernelWeights, _act, _dense, _linear_kn, _linear_tc, plain_linears
 
 
 class Sp_GalerkinAttention(_KernelWeights):
+    activation_bits = 32         # 8: training keeps the input of the output projection in 8 bits
+
     def __init__(self, dim_hidden, num_head, dim_position, norm_eps, attn_droprate, fc_droprate, xavier, diagonal,
                  symmetric) -> None:
         super().__init__()
@@ -109,6 +111,9 @@ def _attention_forward_train(self, Q: Tensor, K: Tensor, V: Tensor, position: Te
                                                              position, self.norm_eps, H, dh, dp)
     X = multihead_galerkin_attention_cccr_cuda(q, k, v)                  # [N, H, S, d_pos + d_head]
     X = X.transpose(1, 2).contiguous().view(N, S, H * (dp + dh))
+    if self.activation_bits == 8 and plain_linears(self._watch, self, self.fc_layer):
+        from ..extension.bind.checkpoint8 import linear8
+        return linear8(X, self.fc_layer.weight, self.fc_layer.bias)
     return self.fc_layer(X)
 
 
@@ -198,7 +203,7 @@ class Sp_EncoderLayer(_KernelWeights):
         """Whether the fused training layer stands for this one: its widths and activation, the modules' own linear layers, nothing
         that watches or alters their calls or the gradients through them."""
         a, f = self.attention_layer, self.ffn_layer
-        if not self.fusable or f.activation != 'relu':
+        if not self.fusable or f.activation != 'relu' or a.activation_bits != 32 or f.activation_bits != 32:
             return False
         linears = (a.fc_layer, f.layer1, f.layer2)
         return (all(type(l) is torch.nn.Linear and l.bias is not None for l in linears)

@@ -121,7 +121,9 @@ def _normalizer_affine(normalizer, r: int, device):
 class Sp_GalerkinTransformer2D(torch.nn.Module):
     """Darcy Galerkin Transformer forward: down-scaler -> encoder layers -> up-scaler -> spectral regressor ->
     de-normalisation -> Dirichlet frame (network/sp_model.py:67-113).  cfg carries the keys of the reference's
-    config (config/darcy_config.yaml) plus 'resolution_size' and 'target_normalizer'."""
+    config (config/darcy_config.yaml) plus 'resolution_size' and 'target_normalizer', and optionally 'num_norm_group' (group
+    normalisation in the scalers' convolution blocks) and 'activation_bits' (8: training keeps the inputs of normalisations and
+    dense layers in 8 bits)."""
 
     def __init__(self, cfg) -> None:
         super().__init__()
@@ -129,16 +131,22 @@ class Sp_GalerkinTransformer2D(torch.nn.Module):
         self.boundary_condition = cfg['boundary_condition']
         self.normalizer = cfg.get('target_normalizer')
         self.down_scaler = DownScaler2D(cfg['resolution_size'], cfg['dim_node'], cfg['dim_hidden'], cfg['drop_downscaler'],
-                                        cfg['acti_downscaler'])
+                                        cfg['acti_downscaler'], cfg.get('num_norm_group', 0))
         self.encoder_mixer = Sp_EncoderMixer(
             cfg['num_encoder_layer'], cfg['dim_hidden'], cfg['num_head'], cfg['dim_position'], cfg['attn_norm_eps'],
             cfg['drop_encoder_attn'], cfg['drop_encoder_attn_fc'], cfg['attn_xavier'], cfg['attn_diagonal'],
             cfg['attn_symmetric'], cfg['dim_encoder_ffn'], cfg['drop_encoder_ffn'], cfg['acti_encoder_ffn'])
         self.up_scaler = UpScaler2D(cfg['resolution_size'], cfg['dim_hidden'], cfg['dim_hidden'], cfg['drop_upscaler'],
-                                    cfg['acti_upscaler'])
+                                    cfg['acti_upscaler'], cfg.get('num_norm_group', 0))
         self.decoder_regressor = Sp_DecoderRegressor(
             cfg['num_decoder_layer'], cfg['dim_hidden'], cfg['dim_target'], cfg['dim_position'], cfg['dim_spatial_hidden'],
             cfg['num_frequence_mode'], cfg['drop_decoder_layer'], cfg['acti_decoder_layer'])
+        bits = cfg.get('activation_bits', 32)
+        if bits not in (8, 32):
+            raise ValueError('activation_bits must be 8 or 32')
+        for m in self.modules():
+            if hasattr(type(m), 'activation_bits'):
+                m.activation_bits = bits
         self._affine = None
         self._plan, self._watch = None, ParameterWatch()
 
@@ -255,7 +263,7 @@ class Sp_GalerkinTransformer2D(torch.nn.Module):
         enc, dec, down, up = self.encoder_mixer.layers, self.decoder_regressor, self.down_scaler, self.up_scaler
         if not (type(dec) is Sp_DecoderRegressor
                 and all(type(l) is Sp_EncoderLayer for l in enc) and all(type(l) is Sp_SpectralConv2D for l in dec.layers)
-                and all(type(c) is ConvResBlock2D for c in (down.conv0, down.conv1, down.conv2, down.conv3, up.conv))
+                and all(type(c) is ConvResBlock2D and c.norm is None for c in (down.conv0, down.conv1, down.conv2, down.conv3, up.conv))
                 and type(up.conv.conv_layer) is torch.nn.Conv2d and type(dec.spatial_fc_layer) is torch.nn.Linear):
             return False
         return (all(l.fusable and l.attention_layer.norm_eps == enc[0].attention_layer.norm_eps
