@@ -19,7 +19,7 @@ class Activation8_Function(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         activation, shape, dtype = ctx.args
-        kept = ops.Checkpoint8(*ctx.saved_tensors, shape, dtype)
+        kept = ops.Checkpoint8._of(*ctx.saved_tensors, shape, dtype)
         return ops.activation8_backward(grad_out.contiguous(), kept, activation), None
 
 
@@ -40,7 +40,7 @@ class Linear8_Function(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dX = torch.matmul(grad_out, weight.to(grad_out.dtype)).to(dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw, db = ops.weight_gradient8(grad_out.contiguous(), ops.Checkpoint8(codes, steps, shape, dtype), column_sums=has_bias)
+            dw, db = ops.weight_gradient8(grad_out.contiguous(), ops.Checkpoint8._of(codes, steps, shape, dtype), column_sums=has_bias)
             dw, db = dw.to(weight.dtype), None if db is None else db.to(weight.dtype)
         return dX, dw, db
 

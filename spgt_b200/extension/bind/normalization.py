@@ -20,7 +20,7 @@ class Group_Norm_Act_Function(torch.autograd.Function):
     def backward(ctx, grad_out):
         weight, bias, stats, *saved = ctx.saved_tensors
         num_groups, activation, shape, dtype = ctx.args
-        X = saved[0] if len(saved) == 1 else ops.Checkpoint8(*saved, shape, dtype)
+        X = saved[0] if len(saved) == 1 else ops.Checkpoint8._of(*saved, shape, dtype)
         dX, dw, db = ops.group_norm_backward(grad_out.contiguous(), X, num_groups, weight, bias, stats, activation)
         return dX, dw if weight is not None else None, db if bias is not None else None, None, None, None, None
 

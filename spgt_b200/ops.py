@@ -25,7 +25,8 @@ def act_code(name) -> int:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream's handle, without the Stream object that torch.cuda.current_stream() makes (5 us of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 class _device:
@@ -791,12 +792,16 @@ DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _dtype(t: Tensor, name: str) -> int:
+    """The type code of a tensor that a kernel can read, or the reason why it cannot."""
+    if isinstance(t, Tensor) and t.is_cuda and t.is_contiguous():
+        code = DTYPE.get(t.dtype)
+        if code is not None:
+            return code
     if not isinstance(t, Tensor):
         raise TypeError(f'{name} must be a torch.Tensor')
     if t.dtype not in DTYPE:
         raise TypeError(f'{name} must be float32, bfloat16 or float16, got {t.dtype}')
     _chk(t, name, t.dtype)
-    return DTYPE[t.dtype]
 
 
 def _aligned(t: Tensor) -> Tensor:
@@ -822,12 +827,16 @@ class Checkpoint8:
         self.codes, self.steps, self.shape, self.dtype = _aligned(codes), steps, torch.Size(shape), dtype
 
     @classmethod
-    def _empty(cls, x: Tensor):
-        self, n = cls.__new__(cls), x.numel()
-        self.shape, self.dtype = x.shape, x.dtype
-        self.codes = torch.empty(n, dtype=torch.int8, device=x.device)
-        self.steps = torch.empty((n + 31) // 32, dtype=torch.uint8, device=x.device)
+    def _of(cls, codes: Tensor, steps: Tensor, shape: torch.Size, dtype):
+        """From tensors that a checkpoint was taken apart into."""
+        self = cls.__new__(cls)
+        self.codes, self.steps, self.shape, self.dtype = codes, steps, shape, dtype
         return self
+
+    @classmethod
+    def _empty(cls, x: Tensor):
+        n = x.numel()
+        return cls._of(x.new_empty(n, dtype=torch.int8), x.new_empty((n + 31) // 32, dtype=torch.uint8), x.shape, x.dtype)
 
     @property
     def device(self):
@@ -841,7 +850,7 @@ class Checkpoint8:
 
 
 def _same(t: Tensor, name: str, shape, device) -> Tensor:
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f'{name} must be {tuple(shape)}, got {tuple(t.shape)}')
     if t.device != device:
         raise ValueError(f'{name} must be on {device}, got {t.device}')
@@ -860,9 +869,10 @@ def compress8(x: Tensor) -> Checkpoint8:
 
 def restore8(kept: Checkpoint8) -> Tensor:
     """The values of a checkpoint, in the type of the tensor it was made from."""
-    with _device(kept.device):
-        out = torch.empty(kept.shape, dtype=kept.dtype, device=kept.device)
-        _call('spgt_restore8', kept.codes.data_ptr(), kept.steps.data_ptr(), None, 0, out.data_ptr(), DTYPE[kept.dtype], out.numel(), _stream())
+    codes = kept.codes
+    with _device(codes.device):
+        out = codes.new_empty(kept.shape, dtype=kept.dtype)
+        _call('spgt_restore8', codes.data_ptr(), kept.steps.data_ptr(), None, 0, out.data_ptr(), DTYPE[kept.dtype], codes.numel(), _stream())
     return out
 
 
@@ -879,9 +889,8 @@ def activation8(x: Tensor, act) -> Tuple[Tensor, Checkpoint8]:
 def activation8_backward(grad_out: Tensor, kept: Checkpoint8, act) -> Tensor:
     """grad_out * act'(kept)."""
     code = _dtype(grad_out, 'grad_out')
-    _same(grad_out, 'grad_out', kept.shape, kept.device)
-    grad_out = _aligned(grad_out)
-    with _device(kept.device):
+    grad_out = _aligned(_same(grad_out, 'grad_out', kept.shape, kept.codes.device))
+    with _device(grad_out.device):
         dx = torch.empty_like(grad_out)
         _call('spgt_restore8', kept.codes.data_ptr(), kept.steps.data_ptr(), grad_out.data_ptr(), act_code(act), dx.data_ptr(), code, dx.numel(), _stream())
     return dx
@@ -891,35 +900,41 @@ def weight_gradient8(grad_out: Tensor, kept: Checkpoint8, column_sums: bool = Tr
     """(grad_out^T kept [N, K], column sums of grad_out [N] or None), fp32, for grad_out [..., N] and a checkpoint of [..., K]: weight and
     bias gradient of a linear layer from its input in 8 bits."""
     code = _dtype(grad_out, 'grad_out')
-    if grad_out.dim() < 1 or len(kept.shape) != grad_out.dim() or grad_out.shape[:-1] != kept.shape[:-1]:
+    if len(kept.shape) < 1 or grad_out.shape[:-1] != kept.shape[:-1] or grad_out.dim() != len(kept.shape):
         raise ValueError('grad_out must be [..., N] for a checkpoint of [..., K]')
-    if grad_out.device != kept.device:
+    if grad_out.device != kept.codes.device:
         raise ValueError('grad_out and the checkpoint must be on the same device')
     grad_out = _aligned(grad_out)
     N, K, rows = grad_out.shape[-1], kept.shape[-1], math.prod(kept.shape[:-1])
-    need = int(lib.spgt_weight_gradient8_workspace_bytes(N, K, rows))
-    if need == 0:
-        raise ValueError(f'unsupported sizes N={N}, K={K}, rows={rows}')
-    with _device(kept.device):
-        dw = torch.empty(N, K, dtype=torch.float32, device=kept.device)
-        db = torch.empty(N, dtype=torch.float32, device=kept.device) if column_sums else None
-        ws = torch.empty(need, dtype=torch.uint8, device=kept.device)
+    with _device(grad_out.device):
+        need = lib.spgt_weight_gradient8_workspace_bytes(N, K, rows)
+        if need == 0:
+            raise ValueError(f'unsupported sizes N={N}, K={K}, rows={rows}')
+        dw = grad_out.new_empty((N, K), dtype=torch.float32)
+        db = grad_out.new_empty(N, dtype=torch.float32) if column_sums else None
+        ws = grad_out.new_empty(need, dtype=torch.uint8)
         _call('spgt_weight_gradient8', grad_out.data_ptr(), code, kept.codes.data_ptr(), kept.steps.data_ptr(), dw.data_ptr(), _p(db), N, K, rows,
               ws.data_ptr(), need, _stream(), kernels=2)
     return dw, db
 
 
 def _norm_sizes(x: Tensor, num_groups: int):
-    if x.dim() < 2:
+    shape = x.shape
+    if len(shape) < 2:
         raise ValueError('x must be [N, ..., C]')
-    N, C = x.shape[0], x.shape[-1]
+    C = shape[-1]
     if C < 1 or num_groups < 1 or C % num_groups:
         raise ValueError(f'{C} channels do not divide into {num_groups} groups')
-    return N, math.prod(x.shape[1:-1]), C, num_groups
+    return shape[0], math.prod(shape[1:-1]), C
 
 
-def _norm_param(t: Optional[Tensor], name: str, C: int, device) -> Optional[Tensor]:
-    return None if t is None else _same(_chk(t, name), name, (C,), device)
+def _norm_param(t: Optional[Tensor], name: str, C: int, device) -> Optional[int]:
+    """A parameter's address."""
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or t.shape != (C,) or t.device != device or not t.is_contiguous():
+        _same(_chk(t, name), name, (C,), device)
+    return t.data_ptr()
 
 
 def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1.0e-5, act=None,
@@ -927,43 +942,48 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optio
     """(act(group_norm(x) * weight + bias), statistics [N, num_groups, 2], x in 8 bits or None) for x [N, ..., C], channels last;
     weight, bias [C] fp32 or None."""
     code = _dtype(x, 'x')
-    N, P, C, G = _norm_sizes(x, num_groups)
-    weight, bias = _norm_param(weight, 'weight', C, x.device), _norm_param(bias, 'bias', C, x.device)
+    N, P, C = _norm_sizes(x, num_groups)
+    device = x.device
+    w, b = _norm_param(weight, 'weight', C, device), _norm_param(bias, 'bias', C, device)
     if not eps >= 0:
         raise ValueError('eps must not be negative')
     x = _aligned(x)
-    with _device(x.device):
-        need = int(lib.spgt_group_norm_workspace_bytes(N, P, C, G, code))
+    with _device(device):
+        need = lib.spgt_group_norm_workspace_bytes(N, P, C, num_groups, code)
         if need == 0:
-            raise ValueError(f'unsupported number of channels C={C}')
-        y, stats = torch.empty_like(x), torch.empty(N, G, 2, dtype=torch.float32, device=x.device)
+            raise ValueError(f'unsupported sizes: {C} channels, {N} samples of {P} pixels')
+        y, stats = torch.empty_like(x), x.new_empty((N, num_groups, 2), dtype=torch.float32)
         kept = Checkpoint8._empty(x) if compress else None
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        _call('spgt_group_norm_fwd', x.data_ptr(), _p(weight), _p(bias), y.data_ptr(), stats.data_ptr(), kept.codes.data_ptr() if compress else None,
-              kept.steps.data_ptr() if compress else None, N, P, C, G, float(eps), act_code(act), code, ws.data_ptr(), need, _stream(),
-              kernels=0 if x.numel() == 0 else 4 if compress and C % 32 else 3)
+        ws = x.new_empty(need, dtype=torch.uint8)
+        _call('spgt_group_norm_fwd', x.data_ptr(), w, b, y.data_ptr(), stats.data_ptr(), kept.codes.data_ptr() if compress else None,
+              kept.steps.data_ptr() if compress else None, N, P, C, num_groups, eps, act_code(act), code, ws.data_ptr(), need, _stream(),
+              kernels=0 if N * P == 0 else 2 if compress and C % 32 else 1)
     return y, stats, kept
 
 
 def group_norm_backward(grad_out: Tensor, x, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, act=None):
     """(dx, dweight [C], dbias [C]) of group_norm for x, the forward's input or a Checkpoint8 of it, and the forward's statistics."""
     code = _dtype(grad_out, 'grad_out')
-    kept = x if isinstance(x, Checkpoint8) else None
-    if kept is None and _dtype(x, 'x') != code:
-        raise TypeError('x and grad_out must have the same type')
-    N, P, C, G = _norm_sizes(grad_out, num_groups)
-    _same(grad_out, 'grad_out', x.shape, x.device)
-    weight, bias = _norm_param(weight, 'weight', C, x.device), _norm_param(bias, 'bias', C, x.device)
-    _same(_chk(stats, 'stats'), 'stats', (N, G, 2), x.device)
-    grad_out, x, stats = _aligned(grad_out), x if kept is not None else _aligned(x), _aligned(stats)
-    with _device(grad_out.device):
-        need = int(lib.spgt_group_norm_bwd_workspace_bytes(N, P, C, G, code))
+    device = grad_out.device
+    N, P, C = _norm_sizes(grad_out, num_groups)
+    if type(x) is Checkpoint8:
+        if x.shape != grad_out.shape or x.codes.device != device:
+            raise ValueError('the checkpoint must be of grad_out\'s shape, on its device')
+        values, codes, steps = None, x.codes.data_ptr(), x.steps.data_ptr()
+    else:
+        if _dtype(x, 'x') != code:
+            raise TypeError('x and grad_out must have the same type')
+        x = _aligned(_same(x, 'x', grad_out.shape, device))
+        values, codes, steps = x.data_ptr(), None, None
+    w, b = _norm_param(weight, 'weight', C, device), _norm_param(bias, 'bias', C, device)
+    stats, grad_out = _aligned(_same(_chk(stats, 'stats'), 'stats', (N, num_groups, 2), device)), _aligned(grad_out)
+    with _device(device):
+        need = lib.spgt_group_norm_bwd_workspace_bytes(N, P, C, num_groups, code)
         if need == 0:
-            raise ValueError(f'unsupported number of channels C={C}')
+            raise ValueError(f'unsupported sizes: {C} channels, {N} samples of {P} pixels')
         dx = torch.empty_like(grad_out)
-        dw, db = (torch.empty(C, dtype=torch.float32, device=dx.device) for _ in range(2))
-        ws = torch.empty(need, dtype=torch.uint8, device=dx.device)
-        _call('spgt_group_norm_bwd', grad_out.data_ptr(), None if kept is not None else x.data_ptr(), kept.codes.data_ptr() if kept is not None else None,
-              kept.steps.data_ptr() if kept is not None else None, _p(weight), _p(bias), stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
-              N, P, C, G, act_code(act), code, ws.data_ptr(), need, _stream(), kernels=0 if dx.numel() == 0 else 4)
+        dw, db = grad_out.new_empty(C, dtype=torch.float32), grad_out.new_empty(C, dtype=torch.float32)
+        ws = grad_out.new_empty(need, dtype=torch.uint8)
+        _call('spgt_group_norm_bwd', grad_out.data_ptr(), values, codes, steps, w, b, stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+              N, P, C, num_groups, act_code(act), code, ws.data_ptr(), need, _stream(), kernels=0 if N * P == 0 else 1)
     return dx, dw, db
