@@ -11,32 +11,23 @@
 // Variances are sums of squared distances from a mean throughout: within a thread's vectors, then merged with
 // M2 = M2a + M2b + (ma - mb)^2 na nb / (na + nb), so a mean far from zero costs no digits.  All sums have a fixed order.
 //
-// One launch each way.  The work is a list of items, a tile's sums or a tile's results, which blocks take in order through a
-// ticket counter; the block that finishes a sample's last sums merges them and raises the sample's flag, and items that need the
-// flag wait for it.  An item only waits for items before it in the list, and those are in the hands of blocks that run, so every
-// wait ends however few blocks run at a time.  The sums of a unit of samples come one unit before its results: the results'
-// reads of x (and dy) then find it in L2 and the waits are over before they begin.
-// A warp of its own takes the items and copies their vectors, in chunks of a few rows, into a ring in shared memory, ahead of the
-// threads that compute: the latencies of the counters, the statistics and the merges are not the memory's.
+// Each way is a pass for the sums, which leaves a word per group and tile, and a pass for the results, whose blocks merge their
+// sample's words themselves.  Both read x, so they take turns over units of samples that stay in L2 in between: the first pass asks L2
+// to keep what it reads, the second to let go of what it reads and writes.  Launches are chained (common.cuh), which hides their gaps.
 #include "lowp.cuh"
-#include "tc_common.cuh"
 
 namespace spgt {
 
-constexpr int GN_ROWS = 4;              // rows of vectors in a chunk
-constexpr int GN_STAGES = 3;            // chunks in the ring
-constexpr int GN_MAX_WORK = 512;        // computing threads, most
-constexpr int GN_HEADER = 384;          // barriers, flag and tasks before the ring
+constexpr int GN_MAX_WORK = 512;        // threads of a block, most
 
 struct GnShape {
     int64_t L;                  // values of a sample
     int N, C, G, cg;
     int V, K, mult;             // values per vector, vectors per period, periods of channels in one period of vectors
     int R, iters, tiles;        // vector rows a block takes at once, how many times per tile, tiles per sample
-    int work;                   // computing threads; a warp more copies
+    int work;                   // threads
     int lanes;                  // threads that work on a group together
-    int unit, lag;              // samples per unit of the list; units between a unit's sums and its results
-    int items;
+    int unit;                   // samples per unit
 };
 struct GnParams {
     GnShape s;
@@ -46,26 +37,22 @@ struct GnParams {
     int8_t* out_codes; uint8_t* out_steps;
     const float *w, *b;
     float2* stats;              // [N][G] mean, 1 / sqrt(var + eps)
-    float4* partial;            // [N][tiles][G] count, mean, M2
-    float2 *chan, *sums;        // [N][tiles][C], [N][C]: sum dz, sum dz xh
-    float2* means;              // [N][G]: means of w dz and w dz xh
-    int *ticket, *samples, *count, *flag;   // zero at launch: next item, samples merged; [N] tiles summed, [N] merged
+    float2* words;              // [N][tiles][G] a tile's mean and M2, or its sums of w dz and w dz xh
+    float2* chan;               // [N][tiles][C]: sum dz, sum dz xh
     float *dw, *db;
     float eps;
-    int act;
+    int act, first;             // first: sample of the unit
 };
 
-// An item as the copying warp hands it to the computing threads, in shared memory.
+// Where a block's tile lies.
 struct GnTask {
     int64_t base, first;        // offsets of the tile's first vector and of its sample
     int n, tile, left;          // left: vectors of the tile
     int head, head_here, tail_here;      // single values before the sample's first vector; those this tile takes, before and after
-    int kind;                   // 0 behind the list's end, 1 sums, 2 results
-    int pad;
 };
-template <int V> __device__ __forceinline__ GnTask gn_task(const GnShape& s, int n, int tile, bool sums) {
+template <int V> __device__ __forceinline__ GnTask gn_task(const GnShape& s, int n, int tile) {
     GnTask t;
-    t.n = n; t.tile = tile; t.kind = sums ? 1 : 2;
+    t.n = n; t.tile = tile;
     t.first = n * s.L;
     t.head = (int)((uint32_t)(-t.first) & (uint32_t)(V - 1));
     if (t.head > s.L) t.head = (int)s.L;
@@ -76,13 +63,10 @@ template <int V> __device__ __forceinline__ GnTask gn_task(const GnShape& s, int
     t.tail_here = tile == s.tiles - 1 ? (int)(s.L - t.head - nv * V) : 0;
     return t;
 }
-// A computing thread's place: in a row of vectors, and in the ring.
+// A thread's place in the rows of vectors.
 struct GnThread {
     int row, col, mine, period;
     bool active;
-    int at = 0, item = 0;       // chunks and items taken
-    bool alive = true;          // false once a wait gave up: the thread goes on to the block's next barriers without data, and the
-                                // block ends together before its next item
     __device__ __forceinline__ GnThread(const GnShape& s) {
         row = threadIdx.x / s.K; col = threadIdx.x - row * s.K;
         active = row < s.R; mine = threadIdx.x; period = s.R * s.K;
@@ -113,210 +97,127 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     return v;
 }
 
-__device__ int g_gn_status = 0;
-
-// ---- the list of items ---------------------------------------------------------------------------------------------------------
-// lag 1: sums of unit 0, then for each unit the next one's sums and its results in turn; lag 0: each unit's sums, then its results
-// from the last tile to the first, which are the ones still in L2.
-struct GnItem { int n, tile; bool sums; };
-__device__ __forceinline__ GnItem gn_item(const GnShape& s, int i) {
-    const int full = s.unit * s.tiles, units = (s.N + s.unit - 1) / s.unit;
-    auto place = [&](int u, int k, bool sums) {
-        const int n = k / s.tiles;
-        return GnItem{u * s.unit + n, k - n * s.tiles, sums};
-    };
-    auto size = [&](int u) { const int left = s.N - u * s.unit; return (left < s.unit ? left : s.unit) * s.tiles; };
-    if (s.lag == 0) {
-        const int u = i / (2 * full), k = i - u * 2 * full, n = size(u);
-        return k < n ? place(u, k, true) : place(u, 2 * n - 1 - k, false);
+// L2 policies: kept for the next pass, or let go.
+__device__ __forceinline__ uint64_t gn_keep() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t gn_drop() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+template <class T> __device__ __forceinline__ uint4 gn_raw(const T* p, uint64_t policy) {
+    uint4 v;
+    asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy));
+    return v;
+}
+// f(loaded) for each of the thread's vectors of a tile: load(j) U at a time, j in vectors from the tile's first.
+template <int U, class L, class F> __device__ __forceinline__ void gn_vectors(const GnTask& t, const GnThread& me, L&& load, F&& f) {
+    if (!me.active) return;
+    int j = me.mine;
+    for (; j + (U - 1) * me.period < t.left; j += U * me.period) {
+        decltype(load(0)) r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u] = load(j + u * me.period);
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(j + u * me.period, r[u]);
     }
-    if (i < full) return place(0, i, true);                                  // (the first unit is a whole one, or all)
-    i -= full;
-    const int last = units > 1 ? (units - 2) * 2 * full + full + size(units - 1) : 0;      // where the last unit's results begin
-    if (i >= last) return place(units - 1, i - last, false);
-    const int u = i / (2 * full), k = i - u * 2 * full, next = size(u + 1);   // results of u, sums of u + 1 in turn
-    if (k < 2 * next) return (k & 1) ? place(u, k >> 1, false) : place(u + 1, k >> 1, true);
-    return place(u, k - next, false);
+    for (; j < t.left; j += me.period) f(j, load(j));
 }
-// ---- the ring -----------------------------------------------------------------------------------------------------------------
-struct GnRing {
-    uint8_t* smem; uint32_t bars; int stage_bytes;
-    GnTask* task;               // [stages + 1] items in order: the one being computed and those that have a chunk in the ring
-    volatile int* abort_flag;
-    __device__ __forceinline__ uint32_t full(int s) const { return bars + 8u * s; }
-    __device__ __forceinline__ uint32_t empty(int s) const { return bars + 8u * (GN_STAGES + s); }
-};
-// Copying: `bytes` (a multiple of 16, from a 16-byte boundary) of up to two tensors per chunk.
-__device__ __forceinline__ void gn_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void gn_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// One thread: takes items and fills the ring with their chunks, of `a` and, if not NULL, `b`.  Ends with the list or with the block's
-// abort flag, when what it has copied has arrived.
-template <class T> __device__ __forceinline__ void gn_produce(const GnParams& p, const GnRing& r, const T* a, const T* b) {
-    constexpr int V = Pack<T>::N;
-    const GnShape& s = p.s;
-    const int chunk = s.R * s.K * GN_ROWS;
-    int issued = 0, st = 0, slot = 0;
-    uint32_t phase = 1;
-    for (bool more = true; more;) {
-        const int i = atomicAdd(p.ticket, 1);
-        GnTask t = {};
-        if (i < s.items) {
-            const GnItem item = gn_item(s, i);
-            t = gn_task<V>(s, item.n, item.tile, item.sums);
-        } else more = false;
-        int j = 0;
-        do {                                                                // (a tile without vectors: an empty chunk)
-            const int n = t.left - j < chunk ? t.left - j : chunk;
-            if (!mbar_wait(r.empty(st), phase, r.abort_flag, 121, &g_gn_status)) { more = false; break; }
-            if (j == 0) r.task[slot] = t;
-            const uint32_t bytes = (uint32_t)n * 16u, dst = smem_u32(r.smem) + st * r.stage_bytes;
-            gn_expect(r.full(st), b ? 2 * bytes : bytes);
-            if (bytes) {
-                gn_copy(dst, a + t.base + (int64_t)j * V, bytes, r.full(st));
-                if (b) gn_copy(dst + chunk * 16, b + t.base + (int64_t)j * V, bytes, r.full(st));
-            }
-            ++issued;
-            if (++st == GN_STAGES) { st = 0; phase ^= 1u; }
-            j += chunk;
-        } while (j < t.left);
-        slot = slot == GN_STAGES ? 0 : slot + 1;
-    }
-    int ignored = 0;
-    for (int k = issued > GN_STAGES ? issued - GN_STAGES : 0; k < issued; ++k)
-        mbar_wait(r.full(k % GN_STAGES), (uint32_t)(k / GN_STAGES & 1), &ignored, 122, &g_gn_status);
-}
-__device__ __forceinline__ bool gn_chunk(const GnRing& r, GnThread& me) {
-    if (!mbar_wait(r.full(me.at % GN_STAGES), (uint32_t)(me.at / GN_STAGES & 1), r.abort_flag, 123, &g_gn_status)) me.alive = false;
-    return me.alive;
-}
-__device__ __forceinline__ void gn_free(const GnRing& r, GnThread& me) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(r.empty(me.at % GN_STAGES));
-    ++me.at;
-}
-// barriers of the computing threads
-__device__ __forceinline__ void gn_sync(int work) { asm volatile("bar.sync 1, %0;" ::"r"(work) : "memory"); }
-
-__device__ __forceinline__ bool gn_all(bool v, int work) {
-    uint32_t all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)v), "r"(work) : "memory");
-    return all != 0;
+template <class F> __device__ __forceinline__ void gn_with_act(int act, F&& f) {
+    if (act == SPGT_ACT_SILU) f(std::integral_constant<int, SPGT_ACT_SILU>{});
+    else if (act == SPGT_ACT_RELU) f(std::integral_constant<int, SPGT_ACT_RELU>{});
+    else if (act == SPGT_ACT_SILU2) f(std::integral_constant<int, SPGT_ACT_SILU2>{});
+    else f(std::integral_constant<int, SPGT_ACT_NONE>{});
 }
 
-// One more tile of sample n is summed: whether it was the last.  What the block wrote before is then visible to whoever sees it so.
-__device__ __forceinline__ bool gn_last(int* count, int of, int* slot, int work) {
-    gn_sync(work);
-    if (threadIdx.x == 0) {
-        __threadfence();
-        *slot = atomicAdd(count, 1) == of - 1;
-        __threadfence();
-    }
-    gn_sync(work);
-    return *slot != 0;
-}
-__device__ __forceinline__ void gn_raise(int* flag, int work) {
-    gn_sync(work);
-    if (threadIdx.x == 0) {
-        __threadfence();
-        asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(flag) : "memory");
-    }
-}
-// Waits for a sample's flag, two seconds at most.
-__device__ __forceinline__ bool gn_wait(const int* flag, int* slot, volatile int* abort_flag, int work) {
-    if (threadIdx.x == 0) {
-        int v = 0;
-        unsigned long long t0 = 0;
-        for (uint32_t i = 0;; ++i) {
-            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
-            if (v) break;
-            __nanosleep(32);
-            if ((i & 63u) == 0u) {
-                const unsigned long long now = globaltimer_ns();
-                if (i == 0u) t0 = now;
-                else if (now - t0 > TC_WAIT_LIMIT_NS) { *abort_flag = 120; atomicCAS(&g_gn_status, 0, 120); break; }
-            }
-        }
-        *slot = v;
-    }
-    gn_sync(work);
-    return *slot != 0;
-}
-__device__ __forceinline__ float2 gn_load2(const float2* p) { return __ldcg(p); }     // written in this launch: never from L1
-
-// ---- forward statistics -----------------------------------------------------------------------------------------------------------
+// ---- forward: sums -----------------------------------------------------------------------------------------------------------------
 // JOINT: a vector lies in one group (cg a multiple of V, no head), so its V values are one set; else a set per channel.
-template <class T, bool JOINT>
-__device__ __forceinline__ void gn_stats_tile(const GnParams& p, const GnTask& t, const GnRing& ring, GnThread& me, float2* s_set) {
-    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V;        // s_set: [R K S] mean, M2
-    __shared__ float s_one[2 * V];
-    __shared__ int s_one_group[2 * V];
+template <class T, bool JOINT> __global__ void __launch_bounds__(GN_MAX_WORK) gn_stats_kernel(const GnParams p) {
+    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V, U = 4, B = 2;     // vectors to a merge, merges to a batch of loads
+    extern __shared__ float2 s_set[];                       // [R K S] mean, M2
+    __shared__ float one[2 * V];
+    __shared__ int one_group[2 * V];
+    pdl_launch_next();
     const GnShape& s = p.s;
+    const int n_in = blockIdx.x / s.tiles;
+    const GnTask t = gn_task<V>(s, p.first + n_in, blockIdx.x - n_in * s.tiles);
+    const GnThread me(s);
     const int period = me.period, mine = me.mine, singles = t.head_here + t.tail_here;
-    if (threadIdx.x < singles) {                            // sets of one
-        const int64_t at = gn_single(t, s, threadIdx.x);
-        s_one[threadIdx.x] = to_f32(((const T*)p.x)[t.first + at]);
-        s_one_group[threadIdx.x] = (int)(at % s.C) / s.cg;
-    }
+    const uint64_t keep = gn_keep();
+    const T* x = (const T*)p.x + t.base;
     float mean[S], m2[S], n = 0.0f;
 #pragma unroll
     for (int i = 0; i < S; ++i) mean[i] = m2[i] = 0.0f;
-    // U vectors: their mean, the squared distances from it, then the merge
-    auto take = [&](auto count, const T* x) {
-        constexpr int U = decltype(count)::value;
-        float v[U][V];
+    // M vectors: their mean, the squared distances from it, then the merge
+    auto take = [&](auto count, const uint4* raw) {
+        constexpr int M = decltype(count)::value;
+        float2 v[M][V / 2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_pack(x + u * period * V, v[u]);
-        constexpr float per = JOINT ? (float)(U * V) : (float)U;
+        for (int u = 0; u < M; ++u) unpack_pairs(raw[u], v[u], T{});
+        constexpr float per = JOINT ? (float)(M * V) : (float)M;
         const float total = n + per, fb = __fdividef(per, total), fm = n * fb;
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            float m = 0.0f, q = 0.0f;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if constexpr (JOINT) {
-#pragma unroll
-                    for (int k = 0; k < V; ++k) m += v[u][k];
-                } else m += v[u][i];
-            }
-            m *= 1.0f / per;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if constexpr (JOINT) {
-#pragma unroll
-                    for (int k = 0; k < V; ++k) { const float d = v[u][k] - m; q = fmaf(d, d, q); }
-                } else { const float d = v[u][i] - m; q = fmaf(d, d, q); }
-            }
+        auto merge = [&](int i, float m, float q) {
             const float d = m - mean[i];
             mean[i] = fmaf(d, fb, mean[i]);
             m2[i] += fmaf(d * fm, d, q);
+        };
+        if constexpr (JOINT) {
+            float2 m = v[0][0], q = pair(0.0f);
+#pragma unroll
+            for (int u = 0; u < M; ++u)
+#pragma unroll
+                for (int k = u == 0 ? 1 : 0; k < V / 2; ++k) m = add2(m, v[u][k]);
+            const float mm = (m.x + m.y) * (1.0f / per);
+            const float2 minus = pair(-mm);
+#pragma unroll
+            for (int u = 0; u < M; ++u)
+#pragma unroll
+                for (int k = 0; k < V / 2; ++k) { const float2 d = add2(v[u][k], minus); q = fma2(d, d, q); }
+            merge(0, mm, q.x + q.y);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) {
+                float2 m = v[0][k], q = pair(0.0f);
+#pragma unroll
+                for (int u = 1; u < M; ++u) m = add2(m, v[u][k]);
+                m = mul2(m, pair(1.0f / per));
+                const float2 minus = make_float2(-m.x, -m.y);
+#pragma unroll
+                for (int u = 0; u < M; ++u) { const float2 d = add2(v[u][k], minus); q = fma2(d, d, q); }
+                merge(2 * k, m.x, q.x);
+                merge(2 * k + 1, m.y, q.y);
+            }
         }
         n = total;
     };
-    int left = t.left;
-    const int all = t.left;
-    do {
-        if (!gn_chunk(ring, me)) break;
-        const T* x = reinterpret_cast<const T*>(ring.smem + me.at % GN_STAGES * ring.stage_bytes) + mine * V;
-        if (me.active) {
-            if (left >= GN_ROWS * period) take(std::integral_constant<int, GN_ROWS>{}, x);
-            else for (int u = 0; u * period + mine < left; ++u) take(std::integral_constant<int, 1>{}, x + u * period * V);
-        }
-        left -= GN_ROWS * period;
-        gn_free(ring, me);
-    } while (left > 0);
     if (me.active) {
+        int j = mine;
+        for (; j + (U * B - 1) * period < t.left; j += U * B * period) {
+            uint4 raw[U * B];
+#pragma unroll
+            for (int u = 0; u < U * B; ++u) raw[u] = gn_raw(x + (int64_t)(j + u * period) * V, keep);
+#pragma unroll
+            for (int k = 0; k < B; ++k) take(std::integral_constant<int, U>{}, raw + U * k);
+        }
+        for (; j < t.left; j += period) {
+            const uint4 raw = gn_raw(x + (int64_t)j * V, keep);
+            take(std::integral_constant<int, 1>{}, &raw);
+        }
 #pragma unroll
         for (int i = 0; i < S; ++i) s_set[mine * S + i] = make_float2(mean[i], m2[i]);
     }
-    gn_sync(s.work);
+    if (threadIdx.x < singles) {                            // sets of one
+        const int64_t at = gn_single(t, s, threadIdx.x);
+        one[threadIdx.x] = to_f32(((const T*)p.x)[t.first + at]);
+        one_group[threadIdx.x] = (int)(at % s.C) / s.cg;
+    }
+    __syncthreads();
     // groups, `lanes` threads each
     const int lane = threadIdx.x & (s.lanes - 1), groups = s.work / s.lanes;
-    const int even = all == s.iters * period ? s.iters : 0;      // every thread has as many vectors
+    const int even = t.left == s.iters * period ? s.iters : 0;      // every thread has as many vectors
     const int phase = t.head < s.C ? t.head : t.head % s.C;
     for (int g0 = 0; g0 < s.G; g0 += groups) {
         const int g = g0 + threadIdx.x / s.lanes, per_row = JOINT ? s.cg / V : s.mult * s.cg;
@@ -336,7 +237,7 @@ __device__ __forceinline__ void gn_stats_tile(const GnParams& p, const GnTask& t
             }
             if (singles > 0 && lane == 0)
                 for (int e = 0; e < singles; ++e)
-                    if (s_one_group[e] == g) f(1.0f, make_float2(s_one[e], 0.0f));
+                    if (one_group[e] == g) f(1.0f, make_float2(one[e], 0.0f));
         };
         float cnt = 0.0f, sum = 0.0f, m2 = 0.0f;
         sets([&](float c, float2 e) { cnt += c; sum = fmaf(c, e.x, sum); });
@@ -344,133 +245,125 @@ __device__ __forceinline__ void gn_stats_tile(const GnParams& p, const GnTask& t
         const float mean = cnt > 0.0f ? sum / cnt : 0.0f;
         sets([&](float c, float2 e) { const float d = e.x - mean; m2 += fmaf(c * d, d, e.y); });
         m2 = lanes_sum(m2, s.lanes);
-        if (lane == 0 && g < s.G) p.partial[((int64_t)t.n * s.tiles + t.tile) * s.G + g] = make_float4(cnt, mean, m2, 0.0f);
+        if (lane == 0 && g < s.G) p.words[((int64_t)t.n * s.tiles + t.tile) * s.G + g] = make_float2(mean, m2);
     }
+    pdl_wait();                                             // (see gn_bwd_sums_kernel)
 }
 
-// a sample's statistics from its tiles'
-__device__ __forceinline__ void gn_merge_stats(const GnParams& p, int n) {
+// f(pass, tile, word) for this thread's share of the words of a group of sample n, in order, in two passes with between() in between.
+// Up to GN_HELD words are read at a time, and once for both passes if that is all.
+constexpr int GN_HELD = 6;
+template <class F, class B> __device__ __forceinline__ void gn_words(const GnParams& p, int n, int g, F&& f, B&& between) {
     const GnShape& s = p.s;
-    const int lane = threadIdx.x & (s.lanes - 1), groups = s.work / s.lanes;
-    const float total = (float)(s.L / s.C) * (float)s.cg;
-    for (int g0 = 0; g0 < s.G; g0 += groups) {
-        const int g = g0 + threadIdx.x / s.lanes, tiles = g < s.G ? s.tiles : 0;
-        const float4* e = p.partial + (int64_t)n * s.tiles * s.G + g;
-        float sum = 0.0f, m2 = 0.0f;
-#pragma unroll 8
-        for (int k = lane; k < tiles; k += s.lanes) { const float4 v = __ldcg(e + (int64_t)k * s.G); sum = fmaf(v.x, v.y, sum); }
-        const float mean = lanes_sum(sum, s.lanes) / total;
-#pragma unroll 8
-        for (int k = lane; k < tiles; k += s.lanes) { const float4 v = __ldcg(e + (int64_t)k * s.G); const float d = v.y - mean; m2 += fmaf(v.x * d, d, v.z); }
-        m2 = lanes_sum(m2, s.lanes);
-        if (lane == 0 && g < s.G) p.stats[(int64_t)n * s.G + g] = make_float2(mean, rsqrtf(m2 / total + p.eps));
+    const int lane = threadIdx.x & (s.lanes - 1), tiles = g < s.G ? s.tiles : 0, batch = GN_HELD * s.lanes;
+    const float2* at = p.words + (int64_t)n * s.tiles * s.G + g;
+    float2 v[GN_HELD];
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+        for (int from = lane; from < tiles; from += batch) {
+            if (pass == 0 || s.tiles > batch) {
+#pragma unroll
+                for (int i = 0; i < GN_HELD; ++i)
+                    if (from + i * s.lanes < tiles) v[i] = __ldca(at + (int64_t)(from + i * s.lanes) * s.G);
+            }
+#pragma unroll
+            for (int i = 0; i < GN_HELD; ++i)
+                if (from + i * s.lanes < tiles) f(pass, from + i * s.lanes, v[i]);
+        }
+        if (pass == 0) between();
     }
 }
+// What the results of a sample need, for all groups in s_group [G]: pair(g), a group's, on its first lane.
+template <class F> __device__ __forceinline__ void gn_groups(const GnShape& s, float2* s_group, F&& pair) {
+    const int lane = threadIdx.x & (s.lanes - 1), groups = s.work / s.lanes;
+    for (int g0 = 0; g0 < s.G; g0 += groups) {
+        const int g = g0 + threadIdx.x / s.lanes;
+        const float2 v = pair(g);
+        if (lane == 0 && g < s.G) s_group[g] = v;
+    }
+    __syncthreads();
+}
+// mean and 1 / sqrt(var + eps)
+__device__ __forceinline__ float2 gn_merge_stats(const GnParams& p, const GnTask& t, int g) {
+    const GnShape& s = p.s;
+    const float total = (float)(s.L / s.C) * (float)s.cg;
+    // tiles are whole periods of channels, the first one's head and the last one's end apart
+    const int full = s.R * s.iters * s.mult * s.cg, q = t.head / s.C, rest = t.head - q * s.C - g * s.cg;
+    const int before = q * s.cg + (rest < 0 ? 0 : rest > s.cg ? s.cg : rest);
+    const float end = (float)((s.L / s.C) * s.cg - (int64_t)(s.tiles - 1) * full - before);
+    auto count = [&](int k) { return k == s.tiles - 1 ? end + (s.tiles == 1 ? (float)before : 0.0f) : k == 0 ? (float)(full + before) : (float)full; };
+    float sum = 0.0f, m2 = 0.0f, mean = 0.0f;
+    gn_words(p, t.n, g,
+             [&](int pass, int k, float2 v) {
+                 if (pass == 0) sum = fmaf(count(k), v.x, sum);
+                 else { const float d = v.x - mean; m2 += fmaf(count(k) * d, d, v.y); }
+             },
+             [&] { mean = lanes_sum(sum, s.lanes) / total; });
+    m2 = lanes_sum(m2, s.lanes);
+    return make_float2(mean, rsqrtf(m2 / total + p.eps));
+}
 
-// A thread's channels: y or dx = a function of x - mean with factors that are the channels' or, JOINT, the group's.
+// A thread's channels, z = (x - mean) a + b, from its groups' statistics stats(group); JOINT: one group.
 template <int V, bool JOINT> struct GnChannels {
-    static constexpr int S = JOINT ? 1 : V;
-    float mean[S], a[V], b[V];                              // z = (x - mean) a + b
-    __device__ __forceinline__ GnChannels(const GnParams& p, const GnTask& t, const GnThread& me, const float2* stats) {
+    static constexpr int S = JOINT ? 1 : V / 2;
+    float2 minus[S], a[V / 2], b[V / 2];                    // - mean
+    template <class F> __device__ __forceinline__ GnChannels(const GnParams& p, const GnTask& t, const GnThread& me, F&& stats) {
         float rstd = 0.0f;
-        if constexpr (JOINT) { const float2 st = gn_load2(stats + me.col * V / p.s.cg); mean[0] = st.x; rstd = st.y; }
+        if constexpr (JOINT) { const float2 st = stats(me.col * V / p.s.cg); minus[0] = pair(-st.x); rstd = st.y; }
         gn_channels<V>(t, me, p.s, [&](int i, int c, int g) {
             float r = rstd;
-            if constexpr (!JOINT) { const float2 st = gn_load2(stats + g); mean[i] = st.x; r = st.y; }
-            a[i] = r * (p.w ? __ldg(p.w + c) : 1.0f);
-            b[i] = p.b ? __ldg(p.b + c) : 0.0f;
+            if constexpr (!JOINT) { const float2 st = stats(g); (i & 1 ? minus[i / 2].y : minus[i / 2].x) = -st.x; r = st.y; }
+            (i & 1 ? a[i / 2].y : a[i / 2].x) = r * (p.w ? __ldg(p.w + c) : 1.0f);
+            (i & 1 ? b[i / 2].y : b[i / 2].x) = p.b ? __ldg(p.b + c) : 0.0f;
         });
     }
-    __device__ __forceinline__ float centred(float x, int i) const { return x - mean[JOINT ? 0 : i]; }
+    __device__ __forceinline__ float2 minus_mean(int i) const { return minus[JOINT ? 0 : i]; }
 };
 
 // ---- forward: y --------------------------------------------------------------------------------------------------------------------
-template <class T, bool JOINT, bool KEEP>
-__device__ __forceinline__ void gn_apply_tile(const GnParams& p, const GnTask& t, const GnRing& ring, GnThread& me) {
+template <class T, bool JOINT, bool KEEP> __global__ void __launch_bounds__(GN_MAX_WORK) gn_apply_kernel(const GnParams p) {
     constexpr int V = Pack<T>::N;
+    extern __shared__ float2 s_group[];
+    pdl_launch_next();
     const GnShape& s = p.s;
-    const float2* stats = p.stats + (int64_t)t.n * s.G;
-    if (threadIdx.x < t.head_here + t.tail_here) {
-        const int64_t at = gn_single(t, s, threadIdx.x);
-        const int c = (int)(at % s.C);
-        const float2 st = gn_load2(stats + c / s.cg);
-        float z[1] = {fmaf(to_f32(((const T*)p.x)[t.first + at]) - st.x, st.y * (p.w ? p.w[c] : 1.0f), p.b ? p.b[c] : 0.0f)};
-        act_values(p.act, z);
-        ((T*)p.out)[t.first + at] = from_f32<T>(z[0]);
-    }
-    const GnChannels<V, JOINT> ch(p, t, me, stats);
-    const int period = me.period, mine = me.mine;
-    int64_t at = t.base + mine * V;
-    int left = t.left;
-    do {
-        if (!gn_chunk(ring, me)) break;
-        const T* x = reinterpret_cast<const T*>(ring.smem + me.at % GN_STAGES * ring.stage_bytes) + mine * V;
-        const bool whole = left >= GN_ROWS * period;
-#pragma unroll
-        for (int u = 0; u < GN_ROWS; ++u) {
-            if (me.active && (whole || u * period + mine < left)) {
-                float v[V];
-                load_pack(x + u * period * V, v);
-                const int64_t o = at + u * period * V;
-                // (C a multiple of 32: the lanes that share a block of the checkpoint take part together)
-                if constexpr (KEEP) q8_store(p.out_codes, p.out_steps, o, v, (Q8_BLOCK / V == 8 ? 0xffu : 0xfu) << (threadIdx.x & 31 & ~(Q8_BLOCK / V - 1)));
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = fmaf(ch.centred(v[i], i), ch.a[i], ch.b[i]);
-                act_values(p.act, v);
-                store_pack((T*)p.out + o, v);
-            }
+    const int n_in = blockIdx.x / s.tiles;
+    // (the last tiles first: they are the ones that L2 has surely kept)
+    const GnTask t = gn_task<V>(s, p.first + n_in, s.tiles - 1 - (int)(blockIdx.x - n_in * s.tiles));
+    const GnThread me(s);
+    const uint64_t drop = gn_drop();
+    pdl_wait();
+    gn_groups(s, s_group, [&](int g) { return gn_merge_stats(p, t, g); });
+    if (t.tile == 0)
+        for (int g = threadIdx.x; g < s.G; g += s.work) p.stats[(int64_t)t.n * s.G + g] = s_group[g];
+    const GnChannels<V, JOINT> ch(p, t, me, [&](int g) { return s_group[g]; });
+    const T* x = (const T*)p.x + t.base;
+    gn_with_act(p.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        if (threadIdx.x < t.head_here + t.tail_here) {
+            const int64_t at = gn_single(t, s, threadIdx.x);
+            const int c = (int)(at % s.C);
+            const float2 st = s_group[c / s.cg];
+            float z[1] = {fmaf(to_f32(((const T*)p.x)[t.first + at]) - st.x, st.y * (p.w ? p.w[c] : 1.0f), p.b ? p.b[c] : 0.0f)};
+            act_values(ACT, z);
+            ((T*)p.out)[t.first + at] = from_f32<T>(z[0]);
         }
-        at += GN_ROWS * period * V;
-        left -= GN_ROWS * period;
-        gn_free(ring, me);
-    } while (left > 0);
-}
-
-// What every block has: the ring, its barriers, and the computing threads' scratch.
-template <class T> __device__ __forceinline__ GnRing gn_ring(const GnParams& p, uint8_t* smem, int tensors) {
-    GnRing r;
-    r.stage_bytes = p.s.R * p.s.K * GN_ROWS * 16 * tensors;
-    r.smem = smem + GN_HEADER;
-    r.bars = smem_u32(smem);
-    r.task = reinterpret_cast<GnTask*>(smem + 64);
-    r.abort_flag = reinterpret_cast<volatile int*>(smem + 48);
-    if (threadIdx.x == 0) {
-        for (int k = 0; k < GN_STAGES; ++k) { mbar_init(r.full(k), 1); mbar_init(r.empty(k), p.s.work >> 5); }
-        *r.abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
-    return r;
-}
-
-template <class T, bool JOINT, bool KEEP> __global__ void __launch_bounds__(GN_MAX_WORK + 32)
-gn_forward_kernel(const GnParams p) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int slot[2];
-    const GnShape& s = p.s;
-    const GnRing ring = gn_ring<T>(p, smem, 1);
-    float2* scratch = reinterpret_cast<float2*>(ring.smem + GN_STAGES * ring.stage_bytes);
-    if (threadIdx.x >= s.work) {
-        if (threadIdx.x == s.work) gn_produce<T>(p, ring, (const T*)p.x, nullptr);
-        return;
-    }
-    for (GnThread me(s);;) {
-        const bool ready = gn_chunk(ring, me);
-        if (!gn_all(ready, s.work)) return;
-        const GnTask& t = ring.task[me.item++ % (GN_STAGES + 1)];
-        if (t.kind == 0) return;
-        if (t.kind == 1) {
-            const int n = t.n;
-            gn_stats_tile<T, JOINT>(p, t, ring, me, scratch);
-            if (gn_last(p.count + n, s.tiles, slot, s.work)) {
-                gn_merge_stats(p, n);
-                gn_raise(p.flag + n, s.work);
+        gn_vectors<4>(t, me, [&](int j) { return gn_raw(x + (int64_t)j * V, drop); }, [&](int j, const uint4& raw) {
+            float2 v[V / 2];
+            unpack_pairs(raw, v, T{});
+            const int64_t o = t.base + (int64_t)j * V;
+            // (C a multiple of 32: the lanes that share a block of the checkpoint take part together)
+            if constexpr (KEEP) {
+                float x[V];
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) { x[2 * i] = v[i].x; x[2 * i + 1] = v[i].y; }
+                q8_store(p.out_codes, p.out_steps, o, x, (Q8_BLOCK / V == 8 ? 0xffu : 0xfu) << (threadIdx.x & 31 & ~(Q8_BLOCK / V - 1)));
             }
-        } else {
-            if (!gn_wait(p.flag + t.n, slot + 1, ring.abort_flag, s.work)) return;
-            gn_apply_tile<T, JOINT, KEEP>(p, t, ring, me);
-        }
-    }
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) v[i] = act_value2<ACT>(fma2(add2(v[i], ch.minus_mean(i)), ch.a[i], ch.b[i]));
+            __stcs(reinterpret_cast<uint4*>((T*)p.out + o), pack_pairs(v, T{}));
+        });
+    });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------------
@@ -478,224 +371,217 @@ template <class T, bool CODES> __device__ __forceinline__ float gn_load_single(c
     if constexpr (CODES) return (float)p.codes[at] * q8_step(p.steps[at >> 5]);
     else return to_f32(((const T*)p.x)[at]);
 }
-
-// f(offset, x, dy) for each of this thread's vectors of a tile.  dy comes through the ring, and x with it; the codes of a checkpoint,
-// which need not begin on a 16-byte boundary, are loaded here, a chunk ahead.
-template <class T, bool CODES, class F>
-__device__ __forceinline__ void gn_bwd_chunks(const GnParams& p, const GnTask& t, const GnRing& ring, GnThread& me, F&& f) {
-    constexpr int V = Pack<T>::N, W = V / 4;
-    const int period = me.period, mine = me.mine;
-    int64_t at = t.base + mine * V;
-    int left = t.left;
-    uint32_t q[CODES ? GN_ROWS : 1][W];
-    uint32_t e[CODES ? GN_ROWS : 1];
-    auto fetch = [&](int64_t from, int n) {
+// A vector of dy with its x, as loaded.
+template <int V, bool CODES> struct GnPair { uint4 d; uint4 x; };
+template <int V> struct GnPair<V, true> { uint4 d; uint32_t q[V / 4]; uint32_t e; };
+template <class T, bool CODES> __device__ __forceinline__ GnPair<Pack<T>::N, CODES> gn_load_pair(const GnParams& p, int64_t at, uint64_t policy) {
+    constexpr int V = Pack<T>::N;
+    GnPair<V, CODES> r;
+    r.d = gn_raw((const T*)p.dy + at, policy);
+    if constexpr (CODES) {
+        if constexpr (V == 4) {
+            asm volatile("ld.global.L2::cache_hint.u32 %0, [%1], %2;" : "=r"(r.q[0]) : "l"(p.codes + at), "l"(policy));
+        } else {
+            asm volatile("ld.global.L2::cache_hint.v2.u32 {%0, %1}, [%2], %3;" : "=r"(r.q[0]), "=r"(r.q[V / 4 - 1]) : "l"(p.codes + at), "l"(policy));
+        }
+        r.e = __ldg(p.steps + (at >> 5));
+    } else {
+        r.x = gn_raw((const T*)p.x + at, policy);
+    }
+    return r;
+}
+// x - mean and dy
+template <class T, bool CODES, bool JOINT, int V> __device__ __forceinline__ void gn_values(const GnPair<V, CODES>& r, const GnChannels<V, JOINT>& ch, float2 (&x)[V / 2], float2 (&d)[V / 2]) {
+    unpack_pairs(r.d, d, T{});
+    if constexpr (CODES) {
+        const float2 step = pair(q8_step(r.e));
 #pragma unroll
-        for (int u = 0; u < GN_ROWS; ++u)
-            if (me.active && u * period + mine < n) {
-                const int64_t o = from + u * period * V;
-                if constexpr (W == 1) q[u][0] = __ldg(reinterpret_cast<const uint32_t*>(p.codes + o));
-                else { const uint2 w = __ldg(reinterpret_cast<const uint2*>(p.codes + o)); q[u][0] = w.x; q[u][W - 1] = w.y; }
-                e[u] = __ldg(p.steps + (o >> 5));
-            }
-    };
-    if constexpr (CODES) fetch(at, left);
-    do {
-        if (!gn_chunk(ring, me)) break;
-        const T* d = reinterpret_cast<const T*>(ring.smem + me.at % GN_STAGES * ring.stage_bytes) + mine * V;
-        const T* x = d + GN_ROWS * period * V;
-        const bool whole = left >= GN_ROWS * period;
+        for (int w = 0; w < V / 4; ++w) {
+            const uint32_t u = r.q[w] ^ 0x80808080u;
 #pragma unroll
-        for (int u = 0; u < GN_ROWS; ++u) {
-            if (me.active && (whole || u * period + mine < left)) {
-                float vd[V], vx[V];
-                load_pack(d + u * period * V, vd);
-                if constexpr (CODES) {
-                    const float step = q8_step(e[u]);
-#pragma unroll
-                    for (int w = 0; w < W; ++w) {
-                        float four[4];
-                        q8_decode(q[u][w], step, four);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) vx[4 * w + i] = four[i];
-                    }
-                } else load_pack(x + u * period * V, vx);
-                f(at + u * period * V, vx, vd);
+            for (int k = 0; k < 2; ++k) {
+                const float2 c = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + 2 * k)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541 + 2 * k)));
+                x[2 * w + k] = fma2(add2(c, pair(-8388736.0f)), step, ch.minus_mean(2 * w + k));      // (code * step is exact)
             }
         }
-        gn_free(ring, me);
-        at += GN_ROWS * period * V;
-        left -= GN_ROWS * period;
-        if constexpr (CODES) fetch(at, left);
-    } while (left > 0);
+    } else {
+        unpack_pairs(r.x, x, T{});
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) x[i] = add2(x[i], ch.minus_mean(i));
+    }
 }
 
-// sums of dz and dz xh of each channel over a tile's pixels
-template <class T, bool JOINT, bool CODES>
-__device__ __forceinline__ void gn_bwd_sums_tile(const GnParams& p, const GnTask& t, const GnRing& ring, GnThread& me, float2* s_sum) {
-    constexpr int V = Pack<T>::N;                           // s_sum: [R][K V]
-    __shared__ float2 s_one[2 * V];
-    __shared__ int s_one_channel[2 * V];
+// sums of dz and dz xh of each channel over a tile's pixels, and of w dz and w dz xh of each group
+template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_MAX_WORK) gn_bwd_sums_kernel(const GnParams p) {
+    constexpr int V = Pack<T>::N;
+    extern __shared__ float2 s_sum[];                       // [R][K V]
+    __shared__ float2 one[2 * V];
+    __shared__ int one_channel[2 * V];
+    pdl_launch_next();
     const GnShape& s = p.s;
+    const int n_in = blockIdx.x / s.tiles;
+    const GnTask t = gn_task<V>(s, p.first + n_in, blockIdx.x - n_in * s.tiles);
+    const GnThread me(s);
     const float2* stats = p.stats + (int64_t)t.n * s.G;
     const int singles = t.head_here + t.tail_here;
-    if (threadIdx.x < singles) {
-        const int64_t at = gn_single(t, s, threadIdx.x);
-        const int c = (int)(at % s.C);
-        const float2 st = stats[c / s.cg];
-        const float xm = gn_load_single<T, CODES>(p, t.first + at) - st.x;
-        const float z[1] = {fmaf(xm, st.y * (p.w ? p.w[c] : 1.0f), p.b ? p.b[c] : 0.0f)};
-        float d[1] = {to_f32(((const T*)p.dy)[t.first + at])};
-        act_slopes(p.act, z, d);
-        s_one[threadIdx.x] = make_float2(d[0], d[0] * xm);
-        s_one_channel[threadIdx.x] = c;
-    }
-    float A[V], B[V];
+    const uint64_t keep = gn_keep();
+    float2 A[V / 2], B[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = B[i] = 0.0f;
-    const GnChannels<V, JOINT> ch(p, t, me, stats);
-    gn_bwd_chunks<T, CODES>(p, t, ring, me, [&](int64_t, float (&v)[V], float (&d)[V]) {
-        float z[V];
+    for (int i = 0; i < V / 2; ++i) A[i] = B[i] = pair(0.0f);
+    const GnChannels<V, JOINT> ch(p, t, me, [&](int g) { return stats[g]; });
+    gn_with_act(p.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        if (threadIdx.x < singles) {
+            const int64_t at = gn_single(t, s, threadIdx.x);
+            const int c = (int)(at % s.C);
+            const float2 st = stats[c / s.cg];
+            const float xm = gn_load_single<T, CODES>(p, t.first + at) - st.x;
+            const float z[1] = {fmaf(xm, st.y * (p.w ? p.w[c] : 1.0f), p.b ? p.b[c] : 0.0f)};
+            float d[1] = {to_f32(((const T*)p.dy)[t.first + at])};
+            act_slopes(ACT, z, d);
+            one[threadIdx.x] = make_float2(d[0], d[0] * xm);
+            one_channel[threadIdx.x] = c;
+        }
+        gn_vectors<2>(t, me, [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, keep); }, [&](int, const GnPair<V, CODES>& r) {
+            float2 v[V / 2], d[V / 2];
+            gn_values<T, CODES, JOINT, V>(r, ch, v, d);
 #pragma unroll
-        for (int i = 0; i < V; ++i) { v[i] = ch.centred(v[i], i); z[i] = fmaf(v[i], ch.a[i], ch.b[i]); }
-        act_slopes(p.act, z, d);
-#pragma unroll
-        for (int i = 0; i < V; ++i) { A[i] += d[i]; B[i] = fmaf(d[i], v[i], B[i]); }
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 dz = act_slope2<ACT>(fma2(v[i], ch.a[i], ch.b[i]), d[i]);
+                A[i] = add2(A[i], dz);
+                B[i] = fma2(dz, v[i], B[i]);
+            }
+        });
     });
     if (me.active) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s_sum[me.mine * V + i] = make_float2(A[i], B[i]);
+        for (int i = 0; i < V / 2; ++i) {
+            s_sum[me.mine * V + 2 * i] = make_float2(A[i].x, B[i].x);
+            s_sum[me.mine * V + 2 * i + 1] = make_float2(A[i].y, B[i].y);
+        }
     }
-    gn_sync(s.work);
+    __syncthreads();
+    // channels, which go to dw and db, then groups, which dx waits for
     const int phase = t.head < s.C ? t.head : t.head % s.C;
     for (int c = threadIdx.x; c < s.C; c += s.work) {
         float2 sum = make_float2(0.0f, 0.0f);
-        const float2* from = s_sum + (c >= phase ? c - phase : c - phase + s.C);
+        float2* own = s_sum + (c >= phase ? c - phase : c - phase + s.C);
+        const float2* from = own;
         for (int r = 0; r < s.R; ++r, from += s.K * V)
             for (int m = 0; m < s.mult; ++m) { const float2 v = from[m * s.C]; sum.x += v.x; sum.y += v.y; }
         for (int e = 0; e < singles; ++e)
-            if (s_one_channel[e] == c) { sum.x += s_one[e].x; sum.y += s_one[e].y; }
-        p.chan[((int64_t)t.n * s.tiles + t.tile) * s.C + c] = make_float2(sum.x, sum.y * stats[c / s.cg].y);
+            if (one_channel[e] == c) { sum.x += one[e].x; sum.y += one[e].y; }
+        sum.y *= stats[c / s.cg].y;
+        p.chan[((int64_t)t.n * s.tiles + t.tile) * s.C + c] = sum;
+        const float w = p.w ? __ldg(p.w + c) : 1.0f;
+        *own = make_float2(w * sum.x, w * sum.y);           // (in the place of its first row)
     }
-}
-
-// Sums over `count` rows of [count][C]: threads take channels and every `rows`-th row, their sums are added in order; f(channel, sum).
-template <class F> __device__ __forceinline__ void gn_column_sums(const float2* v, int count, int C, int work, float2* s_mem, F&& f) {
-    const int rows = C >= work ? 1 : work / C;
-    for (int c0 = 0; c0 < C; c0 += work) {                  // (one pass unless C is larger than the block)
-        const int r = rows == 1 ? 0 : (int)threadIdx.x / C, c = rows == 1 ? c0 + (int)threadIdx.x : (int)threadIdx.x - r * C;
-        float2 sum = make_float2(0.0f, 0.0f);
-        if (r < rows && c < C)
-#pragma unroll 8
-            for (int k = r; k < count; k += rows) { const float2 e = __ldcg(v + (int64_t)k * C + c); sum.x += e.x; sum.y += e.y; }
-        if (rows > 1) {
-            gn_sync(work);
-            if (r < rows) s_mem[threadIdx.x] = sum;
-            gn_sync(work);
-            if (r == 0)
-                for (int k = 1; k < rows; ++k) { const float2 e = s_mem[k * C + c]; sum.x += e.x; sum.y += e.y; }
-        }
-        if (r == 0 && c < C) f(c, sum);
-    }
-    gn_sync(work);
-}
-// a sample's sums, and its groups' means
-__device__ __forceinline__ void gn_bwd_merge(const GnParams& p, int n, float2* s_mem) {
-    const GnShape& s = p.s;
-    float2* sums = p.sums + (int64_t)n * s.C;
-    gn_column_sums(p.chan + (int64_t)n * s.tiles * s.C, s.tiles, s.C, s.work, s_mem, [&](int c, float2 v) { sums[c] = v; });
+    __syncthreads();
     const int lane = threadIdx.x & (s.lanes - 1), groups = s.work / s.lanes;
-    const float total = (float)(s.L / s.C) * (float)s.cg;
     for (int g0 = 0; g0 < s.G; g0 += groups) {
         const int g = g0 + threadIdx.x / s.lanes;
         float c1 = 0.0f, c2 = 0.0f;
-        for (int k = lane; k < s.cg && g < s.G; k += s.lanes) {
-            const int c = g * s.cg + k;
-            const float2 v = sums[c];                       // (of this block)
-            const float w = p.w ? p.w[c] : 1.0f;
-            c1 = fmaf(w, v.x, c1); c2 = fmaf(w, v.y, c2);
-        }
+        for (int k = lane; k < s.cg && g < s.G; k += s.lanes) { const int c = g * s.cg + k; const float2 v = s_sum[c >= phase ? c - phase : c - phase + s.C]; c1 += v.x; c2 += v.y; }
         c1 = lanes_sum(c1, s.lanes); c2 = lanes_sum(c2, s.lanes);
-        if (lane == 0 && g < s.G) p.means[(int64_t)n * s.G + g] = make_float2(c1 / total, c2 / total);
+        if (lane == 0 && g < s.G) p.words[((int64_t)t.n * s.tiles + t.tile) * s.G + g] = make_float2(c1, c2);
     }
+    // Nothing here needs the results of the unit before, whose blocks may still be at work; but whoever waits for this launch to end
+    // counts on those having ended, too.
+    pdl_wait();
+}
+// means of w dz and w dz xh over a group
+__device__ __forceinline__ float2 gn_bwd_merge(const GnParams& p, const GnTask& t, int g) {
+    const GnShape& s = p.s;
+    const float total = (float)(s.L / s.C) * (float)s.cg;
+    float c1 = 0.0f, c2 = 0.0f;
+    gn_words(p, t.n, g, [&](int pass, int, float2 v) { if (pass == 0) { c1 += v.x; c2 += v.y; } }, [] {});
+    return make_float2(lanes_sum(c1, s.lanes) / total, lanes_sum(c2, s.lanes) / total);
 }
 
-template <class T, bool JOINT, bool CODES>
-__device__ __forceinline__ void gn_bwd_apply_tile(const GnParams& p, const GnTask& t, const GnRing& ring, GnThread& me) {
-    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V;
+template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_MAX_WORK) gn_bwd_apply_kernel(const GnParams p) {
+    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V / 2;
+    extern __shared__ float2 s_group[];
+    pdl_launch_next();
     const GnShape& s = p.s;
+    const int n_in = blockIdx.x / s.tiles;
+    const GnTask t = gn_task<V>(s, p.first + n_in, s.tiles - 1 - (int)(blockIdx.x - n_in * s.tiles));
+    const GnThread me(s);
     const float2* stats = p.stats + (int64_t)t.n * s.G;
-    const float2* means = p.means + (int64_t)t.n * s.G;
-    if (threadIdx.x < t.head_here + t.tail_here) {
-        const int64_t at = gn_single(t, s, threadIdx.x);
-        const int c = (int)(at % s.C);
-        const float2 st = stats[c / s.cg], k = gn_load2(means + c / s.cg);
-        const float xm = gn_load_single<T, CODES>(p, t.first + at) - st.x, a = st.y * (p.w ? p.w[c] : 1.0f);
-        const float z[1] = {fmaf(xm, a, p.b ? p.b[c] : 0.0f)};
-        float d[1] = {to_f32(((const T*)p.dy)[t.first + at])};
-        act_slopes(p.act, z, d);
-        ((T*)p.out)[t.first + at] = from_f32<T>(fmaf(xm, -st.y * st.y * k.y, fmaf(a, d[0], -st.y * k.x)));
+    const uint64_t drop = gn_drop();
+    pdl_wait();
+    gn_groups(s, s_group, [&](int g) { return gn_bwd_merge(p, t, g); });
+    const GnChannels<V, JOINT> ch(p, t, me, [&](int g) { return stats[g]; });
+    float2 k1[S], k2[S];
+    if constexpr (JOINT) {
+        const int g = me.col * V / s.cg;
+        const float2 st = stats[g], k = s_group[g];
+        k1[0] = pair(-st.y * k.x); k2[0] = pair(-st.y * st.y * k.y);
+    } else {
+        gn_channels<V>(t, me, s, [&](int i, int, int g) {
+            const float2 st = stats[g], k = s_group[g];
+            (i & 1 ? k1[i / 2].y : k1[i / 2].x) = -st.y * k.x;
+            (i & 1 ? k2[i / 2].y : k2[i / 2].x) = -st.y * st.y * k.y;
+        });
     }
-    const GnChannels<V, JOINT> ch(p, t, me, stats);
-    float k1[S], k2[S];
-    auto constants = [&](int i, int g) { const float2 st = stats[g], k = gn_load2(means + g); k1[i] = -st.y * k.x; k2[i] = -st.y * st.y * k.y; };
-    if constexpr (JOINT) constants(0, me.col * V / s.cg);
-    else gn_channels<V>(t, me, s, [&](int i, int, int g) { constants(i, g); });
-    gn_bwd_chunks<T, CODES>(p, t, ring, me, [&](int64_t at, float (&v)[V], float (&d)[V]) {
-        float z[V];
+    gn_with_act(p.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        if (threadIdx.x < t.head_here + t.tail_here) {
+            const int64_t at = gn_single(t, s, threadIdx.x);
+            const int c = (int)(at % s.C);
+            const float2 st = stats[c / s.cg], k = s_group[c / s.cg];
+            const float xm = gn_load_single<T, CODES>(p, t.first + at) - st.x, a = st.y * (p.w ? p.w[c] : 1.0f);
+            const float z[1] = {fmaf(xm, a, p.b ? p.b[c] : 0.0f)};
+            float d[1] = {to_f32(((const T*)p.dy)[t.first + at])};
+            act_slopes(ACT, z, d);
+            ((T*)p.out)[t.first + at] = from_f32<T>(fmaf(xm, -st.y * st.y * k.y, fmaf(a, d[0], -st.y * k.x)));
+        }
+        gn_vectors<2>(t, me, [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, drop); }, [&](int j, const GnPair<V, CODES>& r) {
+            float2 v[V / 2], d[V / 2];
+            gn_values<T, CODES, JOINT, V>(r, ch, v, d);
 #pragma unroll
-        for (int i = 0; i < V; ++i) { v[i] = ch.centred(v[i], i); z[i] = fmaf(v[i], ch.a[i], ch.b[i]); }
-        act_slopes(p.act, z, d);
-#pragma unroll
-        for (int i = 0; i < V; ++i) d[i] = fmaf(v[i], k2[JOINT ? 0 : i], fmaf(ch.a[i], d[i], k1[JOINT ? 0 : i]));
-        store_pack((T*)p.out + at, d);
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 dz = act_slope2<ACT>(fma2(v[i], ch.a[i], ch.b[i]), d[i]);
+                d[i] = fma2(v[i], k2[JOINT ? 0 : i], fma2(ch.a[i], dz, k1[JOINT ? 0 : i]));
+            }
+            __stcs(reinterpret_cast<uint4*>((T*)p.out + t.base + (int64_t)j * V), pack_pairs(d, T{}));
+        });
     });
 }
 
-template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_MAX_WORK + 32)
-gn_backward_kernel(const GnParams p) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int slot[2];
-    const GnShape& s = p.s;
-    const GnRing ring = gn_ring<T>(p, smem, CODES ? 1 : 2);
-    float2* scratch = reinterpret_cast<float2*>(ring.smem + GN_STAGES * ring.stage_bytes);
-    if (threadIdx.x >= s.work) {
-        if (threadIdx.x == s.work) gn_produce<T>(p, ring, (const T*)p.dy, CODES ? nullptr : (const T*)p.x);
-        return;
+// dw and db from the tiles' sums [rows][C]: a cluster of eight blocks takes 32 channels, its blocks and their warps a share of the rows
+// each; the first block adds the shares up, in order.
+__global__ void __launch_bounds__(512) gn_params_kernel(const float2* chan, int64_t rows, int C, float* dw, float* db) {
+    __shared__ float2 part[16][32];
+    __shared__ float share[2][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x / 8 * 32 + lane;
+    pdl_launch_next();
+    pdl_wait();
+    float2 sum = make_float2(0.0f, 0.0f);
+    if (c < C)
+#pragma unroll 8
+        for (int64_t k = (blockIdx.x & 7) * 16 + w; k < rows; k += 128) { const float2 v = __ldca(chan + k * C + c); sum.x += v.x; sum.y += v.y; }
+    part[w][lane] = sum;
+    __syncthreads();
+    if (w == 0) {
+        for (int k = 1; k < 16; ++k) { const float2 v = part[k][lane]; sum.x += v.x; sum.y += v.y; }
+        share[0][lane] = sum.x; share[1][lane] = sum.y;
     }
-    for (GnThread me(s);;) {
-        const bool ready = gn_chunk(ring, me);
-        if (!gn_all(ready, s.work)) return;
-        const GnTask& t = ring.task[me.item++ % (GN_STAGES + 1)];
-        if (t.kind == 0) return;
-        if (t.kind == 1) {
-            const int n = t.n;
-            gn_bwd_sums_tile<T, JOINT, CODES>(p, t, ring, me, scratch);
-            if (gn_last(p.count + n, s.tiles, slot, s.work)) {
-                gn_bwd_merge(p, n, scratch);
-                gn_raise(p.flag + n, s.work);
-                // the block that merges the last sample adds up the parameters' gradients
-                if (gn_last(p.samples, s.N, slot, s.work))
-                    gn_column_sums(p.sums, s.N, s.C, s.work, scratch, [&](int c, float2 v) { if (p.db) p.db[c] = v.x; if (p.dw) p.dw[c] = v.y; });
-            }
-        } else {
-            if (!gn_wait(p.flag + t.n, slot + 1, ring.abort_flag, s.work)) return;
-            gn_bwd_apply_tile<T, JOINT, CODES>(p, t, ring, me);
-        }
+    cluster_sync_all();
+    if ((blockIdx.x & 7) == 0 && w == 0) {
+        for (int k = 1; k < 8; ++k) { sum.x += ld_dsmem_f32(&share[0][lane], k); sum.y += ld_dsmem_f32(&share[1][lane], k); }
+        if (c < C && db) db[c] = sum.x;
+        if (c < C && dw) dw[c] = sum.y;
     }
-}
-
-int gn_status(bool reset) {
-    int v = 0;
-    if (reset) return cudaMemcpyToSymbol(g_gn_status, &v, sizeof(int)) == cudaSuccess ? SPGT_OK : SPGT_ERR_LAUNCH;
-    return cudaMemcpyFromSymbol(&v, g_gn_status, sizeof(int)) == cudaSuccess ? v : SPGT_ERR_LAUNCH;
+    cluster_sync_all();                                     // (the others' shared memory is read until here)
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------------
-static int gn_shape(int N, int64_t P, int C, int G, int dtype, GnShape& s, int tensors = 1) {
+// tensors: how many both passes read; codes: one of them as a checkpoint (whose workspace is no larger).
+static int gn_shape(int N, int64_t P, int C, int G, int dtype, int tensors, bool codes, GnShape& s) {
     if (N < 0 || P < 0 || C <= 0 || G <= 0 || C % G || dtype < SPGT_F32 || dtype > SPGT_F16) return SPGT_ERR_SHAPE;
     s = GnShape{};
     s.V = dtype == SPGT_F32 ? 4 : 8;
+    const int value_bytes = codes ? 16 / s.V + 1 : 16 / s.V * tensors;
     int d = s.V;
     while (C % d) d >>= 1;                                  // gcd(C, V): V is a power of two
     s.K = C / d; s.mult = s.V / d;
@@ -705,46 +591,30 @@ static int gn_shape(int N, int64_t P, int C, int G, int dtype, GnShape& s, int t
     s.work = ceil_div(s.R * s.K, 32) * 32;
     s.lanes = 32;
     while (s.lanes > 1 && s.lanes * G > s.work) s.lanes >>= 1;
-    // Tiles of up to 16 rows of vectors (64 KB), fewer where that leaves SMs without a tile, more where a sample would have so many
-    // that merging them takes long.
-    const int64_t rows = ceil_div<int64_t>(s.L / s.V, (int64_t)s.R * s.K);
-    int64_t iters = N > 0 ? rows * N / num_sms() / GN_ROWS * GN_ROWS : 1;
-    iters = iters < GN_ROWS ? GN_ROWS : iters > 16 ? 16 : iters;
-    if (iters < rows / 512) iters = ceil_div<int64_t>(rows / 512, GN_ROWS) * GN_ROWS;
-    s.iters = (int)iters;
-    const int64_t tiles = rows > iters ? ceil_div<int64_t>(rows, iters) : 1;
-    if (tiles * (N > 0 ? N : 1) > 0x30000000) return SPGT_ERR_SHAPE;
+    // Units of 96 MB of what is read: fewer launches against more of it found in L2 (64 x 106 x 106 x 128 fp32: units of 48 / 64 / 96 / 112
+    // MB 188 / 179 / 178 / 190 us; 16 samples backward 94 / 100 / 74 / 83).
+    const int64_t bytes = s.L * value_bytes, unit = bytes > 0 ? ((int64_t)96 << 20) / bytes : 1;
+    s.unit = (int)(unit < 1 ? 1 : unit > (N > 0 ? N : 1) ? (N > 0 ? N : 1) : unit);
+    // As many tiles as blocks run at a time, so that a pass is one wave and its blocks end together; no tile of less than four rows of
+    // vectors, nor less than twice the words that a block of the second pass merges.
+    const int64_t rows = ceil_div<int64_t>(s.L / s.V, (int64_t)s.R * s.K), resident = (int64_t)num_sms() * (s.work > 256 ? 1 : s.V == 8 ? 2 : 4);
+    int64_t tiles = resident / s.unit;
+    while (tiles > 1 && tiles * tiles * 16 * G > bytes) tiles = tiles * 7 / 8;
+    if (tiles > rows / 4) tiles = rows / 4;
+    if (tiles < 1) tiles = 1;
+    s.iters = (int)(rows > tiles ? ceil_div(rows, tiles) : 1);
+    tiles = rows > s.iters ? ceil_div<int64_t>(rows, s.iters) : 1;
+    if (tiles * (N > 0 ? N : 1) > 0x7fffffff) return SPGT_ERR_SHAPE;
     s.tiles = (int)tiles;
-    // Units of 24 MB of what is read, which is more than the blocks that run at a time hold; where two units and their results would
-    // not stay in L2, each unit's results follow its sums.
-    const int64_t bytes = s.L * (16 / s.V) * tensors, unit = bytes > 0 ? ceil_div<int64_t>((int64_t)24 << 20, bytes) : 1;
-    s.unit = (int)(unit > (N > 0 ? N : 1) ? (N > 0 ? N : 1) : unit);
-    s.lag = s.unit * bytes <= ((int64_t)40 << 20) ? 1 : 0;
-    s.items = 2 * N * s.tiles;
     return SPGT_OK;
 }
-
-
-// Workspace: the counters, which a launch finds zero, then what the tiles leave.
-static inline size_t gn_counters(int N) { return ((size_t)(2 * (int64_t)N + 4) * sizeof(int) + 15) / 16 * 16; }
-static inline int gn_begin(GnParams& p, void* workspace, cudaStream_t st) {
-    if (cudaError_t e = cudaMemsetAsync(workspace, 0, gn_counters(p.s.N), st)) { g_last_cuda_error = (int)e; (void)cudaGetLastError(); return SPGT_ERR_LAUNCH; }
-    p.ticket = (int*)workspace; p.samples = p.ticket + 1; p.count = p.ticket + 4; p.flag = p.count + p.s.N;
-    return SPGT_OK;
-}
-static inline size_t gn_smem(const GnShape& s, int tensors, int sets) {
-    return GN_HEADER + (size_t)s.R * s.K * (GN_STAGES * GN_ROWS * 16 * tensors + sets * sizeof(float2));
-}
-static inline unsigned gn_grid(const GnShape& s) {
-    const int most = num_sms() * 4;
-    return (unsigned)(s.items < most ? s.items : most);
-}
-
-template <void (*KERNEL)(const GnParams)> static int gn_launch(const GnParams& p, size_t smem, cudaStream_t st) {
+template <void (*KERNEL)(const GnParams)> static int gn_launch(GnParams p, int first, size_t smem, cudaStream_t st) {
     static SmemOptIn configured;
-    if (int e = smem_opt_in(KERNEL, smem, configured)) return e;
-    KERNEL<<<gn_grid(p.s), p.s.work + 32, smem, st>>>(p);
-    return launch_status();
+    if (smem > 48 * 1024)
+        if (int e = smem_opt_in(KERNEL, smem, configured)) return e;
+    p.first = first;
+    const int samples = p.s.N - first < p.s.unit ? p.s.N - first : p.s.unit;
+    return launch_chained(KERNEL, dim3((unsigned)((int64_t)samples * p.s.tiles)), p.s.work, smem, st, p);
 }
 
 }  // namespace spgt
@@ -753,20 +623,20 @@ using namespace spgt;
 
 extern "C" size_t spgt_group_norm_workspace_bytes(int N, int64_t P, int C, int G, int dtype) {
     GnShape s;
-    if (gn_shape(N, P, C, G, dtype, s)) return 0;
-    return gn_counters(N) + (size_t)s.N * s.tiles * s.G * sizeof(float4);
+    if (gn_shape(N, P, C, G, dtype, 1, false, s)) return 0;
+    return (size_t)s.N * s.tiles * s.G * sizeof(float2) + 16;
 }
 extern "C" size_t spgt_group_norm_bwd_workspace_bytes(int N, int64_t P, int C, int G, int dtype) {
     GnShape s;
-    if (gn_shape(N, P, C, G, dtype, s)) return 0;
-    return gn_counters(N) + (((size_t)s.N * s.tiles + s.N) * s.C + (size_t)N * G) * sizeof(float2);
+    if (gn_shape(N, P, C, G, dtype, 2, false, s)) return 0;
+    return (size_t)s.N * s.tiles * (s.G + s.C) * sizeof(float2) + 16;
 }
 
 extern "C" int spgt_group_norm_fwd(const void* x, const float* w, const float* b, void* y, float* stats, int8_t* codes, uint8_t* steps,
                                    int N, int64_t P, int C, int G, float eps, int act, int dtype, void* workspace, size_t workspace_bytes,
                                    spgt_stream_t stream) {
     GnParams p{};
-    if (int e = gn_shape(N, P, C, G, dtype, p.s)) return e;
+    if (int e = gn_shape(N, P, C, G, dtype, 1, false, p.s)) return e;
     if (act < SPGT_ACT_NONE || act > SPGT_ACT_SILU2) return SPGT_ERR_SHAPE;
     if (N == 0 || P == 0) return SPGT_OK;
     if (!x || !y || !stats || !workspace || !codes != !steps) return SPGT_ERR_NULL;
@@ -774,21 +644,24 @@ extern "C" int spgt_group_norm_fwd(const void* x, const float* w, const float* b
     if (!aligned16(x) || !aligned16(y) || !aligned16(stats) || !aligned16(workspace) || (codes && !aligned16(codes))) return SPGT_ERR_ALIGN;
     const GnShape& s = p.s;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (int e = gn_begin(p, workspace, st)) return e;
+    p.words = (float2*)workspace;
     p.x = x; p.out = y; p.w = w; p.b = b; p.stats = (float2*)stats; p.eps = eps; p.act = act;
-    p.partial = (float4*)((char*)workspace + gn_counters(N));
     p.out_codes = codes; p.out_steps = steps;
     const bool joint = s.cg % s.V == 0, keep = codes && C % Q8_BLOCK == 0;
-    const size_t smem = gn_smem(s, 1, joint ? 1 : s.V);
     // (the checkpoint where blocks of 32 values are not whole lanes of the kernel: first, since y may be x)
     if (codes && !keep)
         if (int e = spgt_compress8(x, dtype, SPGT_ACT_NONE, nullptr, codes, steps, N * s.L, stream)) return e;
     return with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
-        if (keep && joint) return gn_launch<gn_forward_kernel<T, true, true>>(p, smem, st);
-        if (keep) return gn_launch<gn_forward_kernel<T, false, true>>(p, smem, st);
-        if (joint) return gn_launch<gn_forward_kernel<T, true, false>>(p, smem, st);
-        return gn_launch<gn_forward_kernel<T, false, false>>(p, smem, st);
+        const size_t sets = (size_t)s.R * s.K * (joint ? 1 : s.V) * sizeof(float2), groups = (size_t)G * sizeof(float2);
+        ChainScope chain;
+        for (int n = 0; n < N; n += s.unit) {
+            if (int e = joint ? gn_launch<gn_stats_kernel<T, true>>(p, n, sets, st) : gn_launch<gn_stats_kernel<T, false>>(p, n, sets, st)) return e;
+            const int e = keep ? (joint ? gn_launch<gn_apply_kernel<T, true, true>>(p, n, groups, st) : gn_launch<gn_apply_kernel<T, false, true>>(p, n, groups, st))
+                               : (joint ? gn_launch<gn_apply_kernel<T, true, false>>(p, n, groups, st) : gn_launch<gn_apply_kernel<T, false, false>>(p, n, groups, st));
+            if (e) return e;
+        }
+        return (int)SPGT_OK;
     });
 }
 
@@ -796,7 +669,7 @@ extern "C" int spgt_group_norm_bwd(const void* dy, const void* x, const int8_t* 
                                    const float* stats, void* dx, float* dw, float* db, int N, int64_t P, int C, int G, int act, int dtype,
                                    void* workspace, size_t workspace_bytes, spgt_stream_t stream) {
     GnParams p{};
-    if (int e = gn_shape(N, P, C, G, dtype, p.s, 2)) return e;
+    if (int e = gn_shape(N, P, C, G, dtype, 2, codes != nullptr, p.s)) return e;
     if (act < SPGT_ACT_NONE || act > SPGT_ACT_SILU2) return SPGT_ERR_SHAPE;
     const cudaStream_t st = (cudaStream_t)stream;
     if (N == 0 || P == 0) {                                 // no pixels: the parameters' gradients are zero
@@ -807,17 +680,37 @@ extern "C" int spgt_group_norm_bwd(const void* dy, const void* x, const int8_t* 
     if (!dy || !dx || !stats || !workspace || (!x && !codes) || (codes && !steps)) return SPGT_ERR_NULL;
     if (workspace_bytes < spgt_group_norm_bwd_workspace_bytes(N, P, C, G, dtype)) return SPGT_ERR_WORKSPACE;
     if (!aligned16(dy) || !aligned16(dx) || !aligned16(stats) || !aligned16(workspace) || (codes ? !aligned16(codes) : !aligned16(x))) return SPGT_ERR_ALIGN;
-    if (int e = gn_begin(p, workspace, st)) return e;
     p.dy = dy; p.x = x; p.codes = codes; p.steps = steps; p.w = w; p.b = b; p.stats = (float2*)stats; p.out = dx; p.dw = dw; p.db = db; p.act = act;
     const GnShape& s = p.s;
-    p.sums = (float2*)((char*)workspace + gn_counters(N));
-    p.means = p.sums + (int64_t)N * C;
-    p.chan = p.means + (int64_t)N * G;
+    p.words = (float2*)workspace;
+    p.chan = p.words + (int64_t)N * s.tiles * G;
     const bool joint = s.cg % s.V == 0;
-    const size_t smem = gn_smem(s, codes ? 1 : 2, s.V);    // (the scratch holds a value per thread of the merges as well)
-    return with_type(dtype, [&](auto zero) {
+    ChainScope chain;
+    const int e = with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
-        if (joint) return codes ? gn_launch<gn_backward_kernel<T, true, true>>(p, smem, st) : gn_launch<gn_backward_kernel<T, true, false>>(p, smem, st);
-        return codes ? gn_launch<gn_backward_kernel<T, false, true>>(p, smem, st) : gn_launch<gn_backward_kernel<T, false, false>>(p, smem, st);
+        const size_t sums = (size_t)s.R * s.K * s.V * sizeof(float2), groups = (size_t)G * sizeof(float2);
+        for (int n = 0; n < N; n += s.unit) {
+            int e = joint ? (codes ? gn_launch<gn_bwd_sums_kernel<T, true, true>>(p, n, sums, st) : gn_launch<gn_bwd_sums_kernel<T, true, false>>(p, n, sums, st))
+                          : (codes ? gn_launch<gn_bwd_sums_kernel<T, false, true>>(p, n, sums, st) : gn_launch<gn_bwd_sums_kernel<T, false, false>>(p, n, sums, st));
+            if (e) return e;
+            e = joint ? (codes ? gn_launch<gn_bwd_apply_kernel<T, true, true>>(p, n, groups, st) : gn_launch<gn_bwd_apply_kernel<T, true, false>>(p, n, groups, st))
+                      : (codes ? gn_launch<gn_bwd_apply_kernel<T, false, true>>(p, n, groups, st) : gn_launch<gn_bwd_apply_kernel<T, false, false>>(p, n, groups, st));
+            if (e) return e;
+        }
+        return (int)SPGT_OK;
     });
+    if (e || !(dw || db)) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ceil_div(C, 32) * 8); cfg.blockDim = dim3(512); cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 8; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    if (const cudaError_t err = cudaLaunchKernelEx(&cfg, gn_params_kernel, (const float2*)p.chan, (int64_t)N * s.tiles, C, dw, db)) {
+        g_last_cuda_error = (int)err; (void)cudaGetLastError();
+        return SPGT_ERR_LAUNCH;
+    }
+    return SPGT_OK;
 }

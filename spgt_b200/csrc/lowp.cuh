@@ -6,7 +6,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include "common.cuh"
+#include "tc_common.cuh"
 
 namespace spgt {
 
@@ -35,9 +35,16 @@ template <class T, int N> __device__ __forceinline__ void store_pack(T* p, const
     for (int i = 0; i < N; ++i) q.v[i] = from_f32<T>(v[i]);
     *reinterpret_cast<Pack<T>*>(p) = q;
 }
-
 // ---- activations of the training operators: a NaN stays a NaN, as in the library's --------------------------------------------
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// sigmoid from the approximate base-2 exponential and reciprocal, relative error below 2^-21 for |z| < 16 (that of the exponent's
+// rounding, z 2^-24, above); results under 2^-126 are zero, and nothing but a NaN gives a NaN.
+__device__ __forceinline__ float sigmoid_f(float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
+__device__ __forceinline__ float silu_value(float z) { return z * sigmoid_f(z); }
 __device__ __forceinline__ float silu_slope(float z) { const float s = sigmoid_f(z); return s * fmaf(z, 1.0f - s, 1.0f); }
 template <int N> __device__ __forceinline__ void act_values(int act, float (&z)[N]) {
     if (act == SPGT_ACT_RELU) {
@@ -45,10 +52,10 @@ template <int N> __device__ __forceinline__ void act_values(int act, float (&z)[
         for (int i = 0; i < N; ++i) z[i] = z[i] < 0.0f ? 0.0f : z[i];
     } else if (act == SPGT_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = silu_f(z[i]);
+        for (int i = 0; i < N; ++i) z[i] = silu_value(z[i]);
     } else if (act == SPGT_ACT_SILU2) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = silu_f(silu_f(z[i]));
+        for (int i = 0; i < N; ++i) z[i] = silu_value(silu_value(z[i]));
     }
 }
 // d *= act'(z)
@@ -61,8 +68,61 @@ template <int N> __device__ __forceinline__ void act_slopes(int act, const float
         for (int i = 0; i < N; ++i) d[i] *= silu_slope(z[i]);
     } else if (act == SPGT_ACT_SILU2) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) d[i] *= silu_slope(silu_f(z[i])) * silu_slope(z[i]);
+        for (int i = 0; i < N; ++i) d[i] *= silu_slope(silu_value(z[i])) * silu_slope(z[i]);
     }
+}
+
+// The same for pairs of values: two fp32 operations per instruction.
+__device__ __forceinline__ float2 pair(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+    const float2 y = mul2(z, pair(-1.4426950408889634f));
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(y.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(y.y));
+    e = add2(e, pair(1.0f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    return r;
+}
+__device__ __forceinline__ float2 silu2(float2 z) { return mul2(z, sigmoid2(z)); }
+__device__ __forceinline__ float2 silu_slope2(float2 z) {
+    const float2 s = sigmoid2(z), t = fma2(s, pair(-1.0f), pair(1.0f));      // 1 - s
+    return fma2(mul2(z, s), t, s);
+}
+template <int ACT> __device__ __forceinline__ float2 act_value2(float2 z) {
+    if constexpr (ACT == SPGT_ACT_RELU) return make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
+    else if constexpr (ACT == SPGT_ACT_SILU) return silu2(z);
+    else if constexpr (ACT == SPGT_ACT_SILU2) return silu2(silu2(z));
+    else return z;
+}
+template <int ACT> __device__ __forceinline__ float2 act_slope2(float2 z, float2 d) {
+    if constexpr (ACT == SPGT_ACT_RELU) return make_float2(z.x > 0.0f ? d.x : (z.x == z.x ? 0.0f : z.x), z.y > 0.0f ? d.y : (z.y == z.y ? 0.0f : z.y));
+    else if constexpr (ACT == SPGT_ACT_SILU) return mul2(d, silu_slope2(z));
+    else if constexpr (ACT == SPGT_ACT_SILU2) return mul2(d, mul2(silu_slope2(silu2(z)), silu_slope2(z)));
+    else return d;
+}
+// 16 bytes of values as pairs
+__device__ __forceinline__ void unpack_pairs(const uint4& r, float2 (&v)[2], float) {
+    v[0] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+    v[1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
+}
+__device__ __forceinline__ void unpack_pairs(const uint4& r, float2 (&v)[4], __nv_bfloat16) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void unpack_pairs(const uint4& r, float2 (&v)[4], __half) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+}
+__device__ __forceinline__ uint4 pack_pairs(const float2 (&v)[2], float) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+}
+__device__ __forceinline__ uint32_t pack_pair(float2 v, __nv_bfloat16) { const __nv_bfloat162 h = __float22bfloat162_rn(v); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t pack_pair(float2 v, __half) { const __half2 h = __float22half2_rn(v); return *reinterpret_cast<const uint32_t*>(&h); }
+template <class T> __device__ __forceinline__ uint4 pack_pairs(const float2 (&v)[4], T t) {
+    return make_uint4(pack_pair(v[0], t), pack_pair(v[1], t), pack_pair(v[2], t), pack_pair(v[3], t));
 }
 
 // ---- 8-bit checkpoints ----------------------------------------------------------------------------------------------------------

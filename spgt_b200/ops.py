@@ -937,6 +937,11 @@ def _norm_param(t: Optional[Tensor], name: str, C: int, device) -> Optional[int]
     return t.data_ptr()
 
 
+def _norm_launches(N: int, sample_bytes: int) -> int:
+    """Two passes for each unit of samples (group_norm.cu: 96 MB of what both read, a sample at least)."""
+    return 0 if N * sample_bytes == 0 else -(-N // max(1, (96 << 20) // sample_bytes)) * 2
+
+
 def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1.0e-5, act=None,
                compress: bool = False):
     """(act(group_norm(x) * weight + bias), statistics [N, num_groups, 2], x in 8 bits or None) for x [N, ..., C], channels last;
@@ -957,7 +962,7 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optio
         ws = x.new_empty(need, dtype=torch.uint8)
         _call('spgt_group_norm_fwd', x.data_ptr(), w, b, y.data_ptr(), stats.data_ptr(), kept.codes.data_ptr() if compress else None,
               kept.steps.data_ptr() if compress else None, N, P, C, num_groups, eps, act_code(act), code, ws.data_ptr(), need, _stream(),
-              kernels=0 if N * P == 0 else 2 if compress and C % 32 else 1)
+              kernels=_norm_launches(N, P * C * x.element_size()) + (compress and C % 32 != 0 and N * P > 0))
     return y, stats, kept
 
 
@@ -985,5 +990,6 @@ def group_norm_backward(grad_out: Tensor, x, num_groups: int, weight: Optional[T
         dw, db = grad_out.new_empty(C, dtype=torch.float32), grad_out.new_empty(C, dtype=torch.float32)
         ws = grad_out.new_empty(need, dtype=torch.uint8)
         _call('spgt_group_norm_bwd', grad_out.data_ptr(), values, codes, steps, w, b, stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
-              N, P, C, num_groups, act_code(act), code, ws.data_ptr(), need, _stream(), kernels=0 if N * P == 0 else 1)
+              N, P, C, num_groups, act_code(act), code, ws.data_ptr(), need, _stream(),
+              kernels=_norm_launches(N, P * C * dx.element_size() * 2 if codes is None else P * C * (dx.element_size() + 1)) + (N * P > 0))
     return dx, dw, db
