@@ -1101,7 +1101,7 @@ namespace spgt {
 int attn_tc_status(); int ffn_tc_status();          // attention_tc.cu, tc_ffn.cu
 int attn_tc_status_reset(); int ffn_tc_status_reset();
 int encoder_kv_status(bool reset); int encoder_out_status(bool reset);     // encoder_kv.cu, encoder_out.cu
-int conv_status(bool reset); int tn_status(bool reset);     // tc_conv.cu, tc_tn.cu
+int conv_status(bool reset); int tn_status(bool reset); int w8_status(bool reset);     // tc_conv.cu, tc_tn.cu, weight_gradient8.cu
 
 // One warp waits on a barrier that nobody arrives at, with a limit of `limit_us` microseconds instead of the two
 // seconds of the production kernels: the wait gives up, latches `code` in the status word and the kernel returns.
@@ -1131,6 +1131,7 @@ extern "C" int spgt_tc_status(void) {
     if (int e = spgt::encoder_out_status(false)) return e;      // 60..76: its second half
     if (int e = spgt::conv_status(false)) return e;             // 80..86: the convolution kernel
     if (int e = spgt::tn_status(false)) return e;               // 90..96: the weight-gradient kernel
+    if (int e = spgt::w8_status(false)) return e;               // 130..134: weight gradients from a checkpoint
     return spgt::ffn_tc_status();               // 21..34: a wait of the fused feed-forward kernel gave up
 }
 
@@ -1142,6 +1143,7 @@ extern "C" int spgt_tc_status_reset(void) {
     if (int e = spgt::encoder_out_status(true)) return e;
     if (int e = spgt::conv_status(true)) return e;
     if (int e = spgt::tn_status(true)) return e;
+    if (int e = spgt::w8_status(true)) return e;
     return spgt::ffn_tc_status_reset();
 }
 
