@@ -4,9 +4,9 @@
 // On the bf16 tensor cores, exactly: a checkpoint's value has seven significant bits and is a bf16 number as it is; dy is the sum of
 // three bf16 numbers (fp32: 8 + 8 + 8 bits, cut off, so nothing overflows), two (fp16) or one (bf16).  All products are exact in fp32.
 // The sums run over the rows, and row-major blocks of rows are what an MMA takes as MN-major operands: nothing is transposed.  Eight
-// warps load blocks of 64 rows, a block ahead, into registers and store them as bf16 parts with the 128-byte swizzle (64 columns of a row
-// are a line); per 16 rows one MMA of 128 x 128 per part.  The accumulate step of an MMA truncates, so after every 64 rows the chain
-// restarts and its result is added to fp32 registers.  Blocks split the rows; their results are added by a second kernel in order.
+// warps copy blocks of 64 rows ahead and store them as bf16 parts with the 128-byte swizzle (64 columns of a row are a line); per 16 rows
+// one MMA of 128 x 128 per part.  The accumulate step of an MMA truncates, so after every 128 rows the chain restarts and its result is
+// added to fp32 registers.  Blocks split the rows; their results are added by a second kernel in order.
 //   warps 0-7 load and convert, 8-15 accumulate, 16 issues the MMAs.  Every wait is a bounded mbarrier poll that records a code on expiry.
 // Floor: rows (N e + 1.03 K) bytes of HBM.
 #include "lowp.cuh"
@@ -15,16 +15,20 @@ namespace spgt {
 
 __device__ int g_w8_status = 0;
 
-constexpr int W8_T = 128, W8_ROWS = 64, W8_STAGES = 2, W8_THREADS = 544;
+constexpr int W8_T = 128, W8_ROWS = 64, W8_STAGES = 2, W8_THREADS = 544, W8_LOADERS = 256;
 constexpr int W8_HALF = W8_ROWS * 128;                      // 64 columns of a block's rows: lines of 128 bytes
 constexpr int W8_PART = 2 * W8_HALF;
-constexpr int W8_BAR = 256;
+constexpr int W8_BAR = 256, W8_CHAIN = 2;                   // blocks of rows that an accumulator sums
 
 template <class T> struct W8Parts { static constexpr int N = 3; };
 template <> struct W8Parts<__half> { static constexpr int N = 2; };
 template <> struct W8Parts<__nv_bfloat16> { static constexpr int N = 1; };
 template <class T> constexpr int w8_stage = (W8Parts<T>::N + 1) * W8_PART;
-template <class T> constexpr int w8_smem = W8_STAGES * w8_stage<T> + W8_BAR;
+// raw values of a block of rows, per loading thread: four units of eight columns of dy, in 16-byte pieces, and of codes
+template <class T> constexpr int w8_pieces = 8 * (int)sizeof(T) / 16;
+template <class T> constexpr int w8_raw = 4 * W8_LOADERS * (16 * w8_pieces<T> + 8);
+template <class T> constexpr int W8_RAWS = sizeof(T) == 4 ? 2 : 4;         // blocks of rows under way
+template <class T> constexpr int w8_smem = W8_STAGES * w8_stage<T> + W8_RAWS<T> * w8_raw<T> + W8_BAR;
 
 struct W8Params {
     const void* dy; const int8_t* codes; const uint8_t* steps;
@@ -34,14 +38,14 @@ struct W8Params {
     int64_t rows;
 };
 
-// Eight consecutive columns of a row, as loaded.
-template <class T> struct W8Dy { uint4 v[sizeof(T) == 4 ? 2 : 1]; };
-struct W8X { uint2 q; uint32_t e; };
-
-// a 16-byte unit of bf16 from eight fp32 bit patterns' upper halves
-__device__ __forceinline__ uint4 w8_upper(const uint32_t (&b)[8]) {
-    return make_uint4(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632), __byte_perm(b[4], b[5], 0x7632), __byte_perm(b[6], b[7], 0x7632));
+// x less its upper half, for pairs: exact, of an infinity a NaN
+__device__ __forceinline__ float2 w8_rest(float2 x) {
+    const float2 up = make_float2(__uint_as_float((__float_as_uint(x.x) & 0xffff0000u) ^ 0x80000000u), __uint_as_float((__float_as_uint(x.y) & 0xffff0000u) ^ 0x80000000u));
+    return add2(x, up);
 }
+__device__ __forceinline__ uint32_t w8_upper(float2 x) { return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632); }
+// a 16-byte unit of bf16 from eight fp32 numbers' upper halves
+__device__ __forceinline__ uint4 w8_upper(const float2 (&b)[4]) { return make_uint4(w8_upper(b[0]), w8_upper(b[1]), w8_upper(b[2]), w8_upper(b[3])); }
 // where unit c (of 16, of eight columns) of row r lies in a part
 __device__ __forceinline__ uint32_t w8_at(int r, int c) { return (uint32_t)((c >> 3) * W8_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
@@ -61,9 +65,9 @@ __device__ __forceinline__ void w8_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 
 // VEC: N and K are multiples of eight, so eight columns of a row are in or out together and start on a boundary of their size.
 template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) weight_gradient8_kernel(const W8Params p) {
-    constexpr int P = W8Parts<T>::N, STAGE = w8_stage<T>;
+    constexpr int P = W8Parts<T>::N, STAGE = w8_stage<T>, RAWS = W8_RAWS<T>, PIECES = w8_pieces<T>, BAR = W8_STAGES * STAGE + RAWS * w8_raw<T>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    const uint32_t base = smem_u32(smem), bars = base + W8_STAGES * STAGE;
+    const uint32_t base = smem_u32(smem), bars = base + BAR;
     if (base & 1023u) {
         if (threadIdx.x == 0) atomicCAS(&g_w8_status, 0, 130);
         return;
@@ -72,8 +76,8 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
     auto st_empty = [&](uint32_t s) { return bars + 8u * (2 + s); };      // [2]
     auto acc_full = [&](uint32_t s) { return bars + 8u * (4 + s); };      // [2]
     auto acc_empty = [&](uint32_t s) { return bars + 8u * (6 + s); };     // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + W8_STAGES * STAGE + 96);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + W8_STAGES * STAGE + 104);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + BAR + 96);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + BAR + 104);
     const int tid = threadIdx.x, warp = (int)tc_uniform(tid >> 5), lane = tid & 31;
     const int tile = blockIdx.y, n0 = tile / p.kt * W8_T, k0 = tile % p.kt * W8_T;
     const int64_t blocks = (p.rows + W8_ROWS - 1) / W8_ROWS, first = blocks * blockIdx.x / p.splits;
@@ -91,128 +95,158 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = tc_uniform(*tmem_slot);
-    float sums[8] = {};
+    float2 sums[4] = {};                                    // of this thread's columns of dy
 
     if (warp < 8) {
-        // ------------------------------------------ load and convert: unit c of rows r0, r0 + 16, ... ------------------------------------------
-        const int c = lane & 15, r0 = warp * 2 + (lane >> 4);
-        const int nc = n0 + c * 8, kc = k0 + c * 8;         // first column of dy and x
-        W8Dy<T> dy[2][4];
-        W8X x[2][4];
-        auto load = [&](int k, W8Dy<T> (&d)[4], W8X (&v)[4]) {
+        // ------------------------------------------ load and convert ------------------------------------------
+        // eight values of dy, in P parts, and of x, of row r and unit c of eight columns
+        auto store = [&](uint8_t* stage, int r, int c, float2 (&b)[4], const float2 (&y)[4]) {
+            const uint32_t at = w8_at(r, c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t r = (first + k) * W8_ROWS + r0 + 16 * i;
-                const bool in = k < mine && r < p.rows;
-                const T* from = (const T*)p.dy + r * p.N + nc;
-                const int64_t at = r * p.K + kc;
+            for (int q = 0; q < P; ++q) {
+                *reinterpret_cast<uint4*>(stage + q * W8_PART + at) = w8_upper(b);
+                if (q + 1 < P) {
 #pragma unroll
-                for (int j = 0; j < (int)(sizeof(d[i].v) / 16); ++j) d[i].v[j] = make_uint4(0, 0, 0, 0);
-                v[i].q = make_uint2(0, 0); v[i].e = 1;
-                if constexpr (VEC) {
-                    if (in && nc < p.N) {
-#pragma unroll
-                        for (int j = 0; j < (int)(sizeof(d[i].v) / 16); ++j) d[i].v[j] = __ldg(reinterpret_cast<const uint4*>(from) + j);
-                    }
-                    if (in && kc < p.K) {
-                        v[i].q = __ldg(reinterpret_cast<const uint2*>(p.codes + at));
-                        v[i].e = __ldg(p.steps + (at >> 5));
-                    }
-                } else if (in) {
-                    T* to = reinterpret_cast<T*>(&d[i]);
-                    uint8_t* codes = reinterpret_cast<uint8_t*>(&v[i].q);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (nc + j < p.N) to[j] = from[j];
-                        if (kc + j < p.K) codes[j] = (uint8_t)p.codes[at + j];
-                    }
-                    // the steps of the eight values: those of the first and, from `from_second` on, of the next block
-                    if (kc < p.K) {
-                        const int64_t blocks32 = (p.rows * p.K + 31) >> 5, b = at >> 5;
-                        v[i].e = p.steps[b] | (b + 1 < blocks32 ? (uint32_t)p.steps[b + 1] << 8 : 0u) | (uint32_t)(32 - (int)(at & 31)) << 16;
-                    }
+                    for (int j = 0; j < 4; ++j) b[j] = w8_rest(b[j]);
                 }
             }
+            *reinterpret_cast<uint4*>(stage + P * W8_PART + at) = pack_pairs(y, __nv_bfloat16{});
         };
-        auto store = [&](int s, const W8Dy<T> (&d)[4], const W8X (&v)[4]) {
-            uint8_t* stage = smem + s * STAGE;
+        uint32_t s = 0, ph = 1;
+        if constexpr (VEC) {
+            // Unit c of rows r0, r0 + 16, ...: each thread copies what it will convert, RAWS blocks of rows ahead, and only waits for itself.
+            const int c = lane & 15, r0 = warp * 2 + (lane >> 4);
+            const int nc = n0 + c * 8, kc = k0 + c * 8;     // first column of dy and x
+            const bool n_in = nc < p.N, k_in = kc < p.K;
+            uint8_t* raw = smem + W8_STAGES * STAGE + tid * 16;
+            uint32_t e[2][4];                               // steps, of this block and the next
+            const int64_t row0 = first * W8_ROWS + r0, dy_row = (int64_t)p.N * (int)sizeof(T), left0 = p.rows - row0;
+            const uint8_t* dy_at = (const uint8_t*)p.dy + row0 * dy_row + (int64_t)nc * (int)sizeof(T);       // of the block to copy
+            const int8_t* codes_at = p.codes + row0 * p.K + kc;
+            int64_t copy_left = left0 < (int64_t)mine * W8_ROWS ? left0 : (int64_t)mine * W8_ROWS;          // rows from this thread's first one
+            int copy_slot = 0;
+            auto copy = [&] {
+                uint8_t* to = raw + copy_slot * w8_raw<T>;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t at = w8_at(r0 + 16 * i, c);
-                if constexpr (P == 1) {
-                    *reinterpret_cast<uint4*>(stage + at) = d[i].v[0];
-                    const uint32_t w[4] = {d[i].v[0].x, d[i].v[0].y, d[i].v[0].z, d[i].v[0].w};
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = 16 * i < copy_left;
+                    const uint8_t* from = in && n_in ? dy_at + 16 * i * dy_row : (const uint8_t*)p.dy;
+                    const int8_t* codes = in && k_in ? codes_at + 16 * i * p.K : p.codes;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) { sums[2 * j] += __uint_as_float(w[j] << 16); sums[2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u); }
-                } else {
-                    float f[8];
-                    if constexpr (P == 3) {
-                        const uint32_t w[8] = {d[i].v[0].x, d[i].v[0].y, d[i].v[0].z, d[i].v[0].w, d[i].v[P == 3].x, d[i].v[P == 3].y, d[i].v[P == 3].z, d[i].v[P == 3].w};
+                    for (int j = 0; j < PIECES; ++j) cp_async_zfill<16>(to + (i * PIECES + j) * (W8_LOADERS * 16), from + 16 * j, in && n_in);
+                    cp_async_zfill<8>(to + 4 * PIECES * (W8_LOADERS * 16) + i * (W8_LOADERS * 8) - tid * 8, codes, in && k_in);
+                }
+                cp_async_commit();
+                dy_at += W8_ROWS * dy_row; codes_at += W8_ROWS * p.K; copy_left -= W8_ROWS;
+                copy_slot = copy_slot == RAWS - 1 ? 0 : copy_slot + 1;
+            };
+            int64_t value_at = row0 * p.K + kc, step_left = copy_left;
+            auto steps = [&](uint32_t (&v)[4]) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = 1;
+                    if (16 * i < step_left && k_in) v[i] = __ldg(p.steps + ((value_at + 16 * i * p.K) >> 5));
+                }
+                value_at += W8_ROWS * p.K; step_left -= W8_ROWS;
+            };
+            int slot = 0;
+            if (mine > 0) {
+#pragma unroll
+                for (int k = 0; k < RAWS; ++k) copy();
+                steps(e[0]);
+            }
+            auto step = [&](uint32_t (&now)[4], uint32_t (&next)[4]) {
+                steps(next);
+                cp_async_wait<RAWS - 1>();
+                if (!mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status)) return false;
+                const uint8_t* from = raw + slot * w8_raw<T>;
+                slot = slot == RAWS - 1 ? 0 : slot + 1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float2 b[4];
+                    if constexpr (PIECES == 2) {
+                        float2 h[2];
+                        unpack_pairs(*reinterpret_cast<const uint4*>(from + 2 * i * (W8_LOADERS * 16)), h, 0.0f);
+                        b[0] = h[0]; b[1] = h[1];
+                        unpack_pairs(*reinterpret_cast<const uint4*>(from + (2 * i + 1) * (W8_LOADERS * 16)), h, 0.0f);
+                        b[2] = h[0]; b[3] = h[1];
                     } else {
-                        const uint32_t w[4] = {d[i].v[0].x, d[i].v[0].y, d[i].v[0].z, d[i].v[0].w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[j])); f[2 * j] = g.x; f[2 * j + 1] = g.y; }
+                        unpack_pairs(*reinterpret_cast<const uint4*>(from + i * (W8_LOADERS * 16)), b, T{});
                     }
-                    uint32_t b[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) { sums[j] += f[j]; b[j] = __float_as_uint(f[j]); }
+                    for (int j = 0; j < 4; ++j) sums[j] = add2(sums[j], b[j]);
+                    const uint2 q = *reinterpret_cast<const uint2*>(from + 4 * PIECES * (W8_LOADERS * 16) + i * (W8_LOADERS * 8) - tid * 8);
+                    const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
+                    const float2 size = pair(q8_step(now[i]));
+                    float2 y[4];
 #pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        *reinterpret_cast<uint4*>(stage + q * W8_PART + at) = w8_upper(b);
-                        if (q + 1 < P) {
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t v = w[j >> 1];
+                        const float2 code = make_float2(__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + 2 * (j & 1))), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7541 + 2 * (j & 1))));
+                        y[j] = mul2(add2(code, pair(-8388736.0f)), size);
+                    }
+                    store(smem + s * STAGE, r0 + 16 * i, c, b, y);
+                }
+                copy();
+                fence_proxy_async();
+                mbar_arrive(st_full(s));
+                if (++s == W8_STAGES) { s = 0; ph ^= 1u; }
+                return true;
+            };
+            for (int k = 0; k < mine; k += 2) {
+                if (!step(e[0], e[1])) break;
+                if (k + 1 < mine && !step(e[1], e[0])) break;
+            }
+            cp_async_wait_all();
+        } else {
+            // Any widths: columns 2 lane, 2 lane + 1 (+ 64) of rows warp, warp + 8, ...
+            for (int k = 0; k < mine; ++k) {
+                if (!mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status)) break;
+                uint8_t* stage = smem + s * STAGE;
+#pragma unroll 1
+                for (int i0 = 0; i0 < 8; i0 += 4) {
+                    float d[4][4], x[4][4];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {           // the rest; none of an infinity
-                                const float h = __uint_as_float(b[j] & 0xffff0000u), g = __uint_as_float(b[j]);
-                                b[j] = __float_as_uint(h == g ? 0.0f : g - h);
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t r = (first + k) * W8_ROWS + warp + 8 * (i0 + i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int col = 2 * lane + (j >> 1) * 64 + (j & 1);
+                            d[i][j] = x[i][j] = 0.0f;
+                            if (r < p.rows && n0 + col < p.N) d[i][j] = to_f32(((const T*)p.dy)[r * p.N + n0 + col]);
+                            if (r < p.rows && k0 + col < p.K) {
+                                const int64_t at = r * p.K + k0 + col;
+                                x[i][j] = (float)p.codes[at] * q8_step(p.steps[at >> 5]);
                             }
                         }
                     }
-                }
-                float2 y[4];
-                const uint32_t w[2] = {v[i].q.x ^ 0x80808080u, v[i].q.y ^ 0x80808080u};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    y[j] = add2(make_float2(__uint_as_float(__byte_perm(w[j >> 1], 0x4b000000u, 0x7540 + 2 * (j & 1))), __uint_as_float(__byte_perm(w[j >> 1], 0x4b000000u, 0x7541 + 2 * (j & 1)))), pair(-8388736.0f));
-                if constexpr (VEC) {
-                    const float2 step = pair(q8_step(v[i].e));
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = warp + 8 * (i0 + i);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) y[j] = mul2(y[j], step);
-                } else {
-                    const float s0 = q8_step(v[i].e & 255u), s1 = q8_step(v[i].e >> 8 & 255u);
-                    const int second = (int)(v[i].e >> 16);
+                        for (int h = 0; h < 2; ++h) {       // 64-column half
+                            uint8_t* at = stage + w8_at(r, 8 * h + (lane >> 2)) + (lane & 3) * 4;
+                            float2 b = make_float2(d[i][2 * h], d[i][2 * h + 1]);
+                            sums[h] = add2(sums[h], b);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        y[j].x = kc + 2 * j < p.K ? y[j].x * (2 * j < second ? s0 : s1) : 0.0f;
-                        y[j].y = kc + 2 * j + 1 < p.K ? y[j].y * (2 * j + 1 < second ? s0 : s1) : 0.0f;
+                            for (int q = 0; q < P; ++q, b = w8_rest(b)) *reinterpret_cast<uint32_t*>(at + q * W8_PART) = w8_upper(b);
+                            *reinterpret_cast<uint32_t*>(at + P * W8_PART) = pack_pair(make_float2(x[i][2 * h], x[i][2 * h + 1]), __nv_bfloat16{});
+                        }
                     }
                 }
-                *reinterpret_cast<uint4*>(stage + P * W8_PART + at) = pack_pairs(y, __nv_bfloat16{});
+                fence_proxy_async();
+                mbar_arrive(st_full(s));
+                if (++s == W8_STAGES) { s = 0; ph ^= 1u; }
             }
-        };
-        load(0, dy[0], x[0]);
-        uint32_t s = 0, ph = 1;
-        bool alive = true;
-        auto step = [&](int k, int cur) {
-            load(k + 1, dy[cur ^ 1], x[cur ^ 1]);
-            if (!mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status)) { alive = false; return; }
-            store(s, dy[cur], x[cur]);
-            fence_proxy_async();
-            mbar_arrive(st_full(s));
-            if (++s == W8_STAGES) { s = 0; ph ^= 1u; }
-        };
-        for (int k = 0; k < mine && alive; k += 2) {
-            step(k, 0);
-            if (k + 1 < mine && alive) step(k + 1, 1);
         }
     } else if (warp == 16) {
         // ------------------------------------------ MMA issuer ------------------------------------------
         if (tc_elect()) {
             uint32_t s = 0, ph = 0;
             for (int k = 0; k < mine; ++k) {
-                const uint32_t buf = (uint32_t)(k & 1), d = tmem_base + buf * W8_T;
-                if (!mbar_wait(acc_empty(buf), (uint32_t)((k >> 1) & 1) ^ 1u, abort_flag, 132, &g_w8_status)) break;
+                const int chain = k / W8_CHAIN, start = k % W8_CHAIN == 0;
+                const uint32_t buf = (uint32_t)(chain & 1), d = tmem_base + buf * W8_T;
+                if (start && !mbar_wait(acc_empty(buf), (uint32_t)((chain >> 1) & 1) ^ 1u, abort_flag, 132, &g_w8_status)) break;
                 if (!mbar_wait(st_full(s), ph, abort_flag, 133, &g_w8_status)) break;
                 tc_fence_after();
                 const uint32_t st = base + s * STAGE;
@@ -221,9 +255,9 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
                 for (int q = P - 1; q >= 0; --q)            // the smallest parts first
 #pragma unroll
                     for (int k16 = 0; k16 < W8_ROWS / 16; ++k16)
-                        w8_mma(d, a + q * (W8_PART >> 4) + k16 * 128, b + k16 * 128, q < P - 1 || k16 > 0 ? 1u : 0u);
+                        w8_mma(d, a + q * (W8_PART >> 4) + k16 * 128, b + k16 * 128, q < P - 1 || k16 > 0 || !start ? 1u : 0u);
                 tc_commit(st_empty(s));
-                tc_commit(acc_full(buf));
+                if (k % W8_CHAIN == W8_CHAIN - 1 || k == mine - 1) tc_commit(acc_full(buf));
                 if (++s == W8_STAGES) { s = 0; ph ^= 1u; }
             }
         }
@@ -236,7 +270,8 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
 #pragma unroll
         for (int j = 0; j < 64; ++j) acc[j] = 0.0f;
         bool alive = true;
-        for (int k = 0; k < mine; ++k) {
+        const int chains = (mine + W8_CHAIN - 1) / W8_CHAIN;
+        for (int k = 0; k < chains; ++k) {
             const uint32_t buf = (uint32_t)(k & 1);
             if (!mbar_wait(acc_full(buf), (uint32_t)((k >> 1) & 1), abort_flag, 134, &g_w8_status)) { alive = false; break; }
             tc_fence_after();
@@ -262,18 +297,24 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256) : "memory");
     }
-    // column sums of dy: 16 threads have a column each; the stages are free
+    // column sums of dy, of several threads each; the stages are free
     if (k0 == 0 && p.db) {
         float* part = reinterpret_cast<float*>(smem);
+        constexpr int SHARES = VEC ? 16 : 8;
         if (warp < 8) {
+            if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) part[(warp * 2 + (lane >> 4)) * W8_T + (lane & 15) * 8 + j] = sums[j];
+                for (int j = 0; j < 8; ++j) part[(warp * 2 + (lane >> 4)) * W8_T + (lane & 15) * 8 + j] = j & 1 ? sums[j / 2].y : sums[j / 2].x;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[warp * W8_T + 2 * lane + (j >> 1) * 64 + (j & 1)] = j & 1 ? sums[j / 2].y : sums[j / 2].x;
+            }
         }
         __syncthreads();
         if (tid < W8_T) {
             float s = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) s += part[k * W8_T + tid];
+            for (int k = 0; k < SHARES; ++k) s += part[k * W8_T + tid];
             p.colpart[((int64_t)blockIdx.x * (gridDim.y / p.kt) + tile / p.kt) * W8_T + tid] = s;
         }
     }
