@@ -7,7 +7,7 @@
 // warps copy blocks of 64 rows ahead and store them as bf16 parts with the 128-byte swizzle (64 columns of a row are a line); per 16 rows
 // one MMA of 128 x 128 per part.  The accumulate step of an MMA truncates, so after every 128 rows the chain restarts and its result is
 // added to fp32 registers.  Blocks split the rows; their results are added by a second kernel in order.
-//   warps 0-7 load and convert, 8-15 accumulate, 16 issues the MMAs.  Every wait is a bounded mbarrier poll that records a code on expiry.
+//   warps 0-7 load and convert, 8-15 accumulate, and the first of those issues the MMAs.  Every wait is a bounded mbarrier poll that records a code on expiry.
 // Floor: rows (N e + 1.03 K) bytes of HBM.
 #include "lowp.cuh"
 
@@ -15,7 +15,7 @@ namespace spgt {
 
 __device__ int g_w8_status = 0;
 
-constexpr int W8_T = 128, W8_ROWS = 64, W8_STAGES = 2, W8_THREADS = 544, W8_LOADERS = 256;
+constexpr int W8_T = 128, W8_ROWS = 64, W8_STAGES = 2, W8_THREADS = 512, W8_LOADERS = 256;
 constexpr int W8_HALF = W8_ROWS * 128;                      // 64 columns of a block's rows: lines of 128 bytes
 constexpr int W8_PART = 2 * W8_HALF;
 constexpr int W8_BAR = 256, W8_CHAIN = 2;                   // blocks of rows that an accumulator sums
@@ -67,6 +67,7 @@ __device__ __forceinline__ void w8_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) weight_gradient8_kernel(const W8Params p) {
     constexpr int P = W8Parts<T>::N, STAGE = w8_stage<T>, RAWS = W8_RAWS<T>, PIECES = w8_pieces<T>, BAR = W8_STAGES * STAGE + RAWS * w8_raw<T>;
     extern __shared__ __align__(1024) uint8_t smem[];
+    pdl_launch_next();                                      // (the second kernel waits for the end of this one)
     const uint32_t base = smem_u32(smem), bars = base + BAR;
     if (base & 1023u) {
         if (threadIdx.x == 0) atomicCAS(&g_w8_status, 0, 130);
@@ -87,7 +88,7 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -99,12 +100,18 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
 
     if (warp < 8) {
         // ------------------------------------------ load and convert ------------------------------------------
-        // eight values of dy, in P parts, and of x, of row r and unit c of eight columns
+        // eight values of dy, in P parts, and of x, of row r: x of unit c of eight columns; dy of the same, or, fp32, of columns 4 c .. + 3
+        // and 64 + 4 c .. + 3, so that the lanes' 16-byte copies are next to each other
         auto store = [&](uint8_t* stage, int r, int c, float2 (&b)[4], const float2 (&y)[4]) {
-            const uint32_t at = w8_at(r, c);
+            const uint32_t at = w8_at(r, c), at4 = w8_at(r, c >> 1) + (c & 1) * 8;
 #pragma unroll
             for (int q = 0; q < P; ++q) {
-                *reinterpret_cast<uint4*>(stage + q * W8_PART + at) = w8_upper(b);
+                if constexpr (P == 3) {
+                    *reinterpret_cast<uint2*>(stage + q * W8_PART + at4) = make_uint2(w8_upper(b[0]), w8_upper(b[1]));
+                    *reinterpret_cast<uint2*>(stage + q * W8_PART + W8_HALF + at4) = make_uint2(w8_upper(b[2]), w8_upper(b[3]));
+                } else {
+                    *reinterpret_cast<uint4*>(stage + q * W8_PART + at) = w8_upper(b);
+                }
                 if (q + 1 < P) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) b[j] = w8_rest(b[j]);
@@ -116,8 +123,8 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
         if constexpr (VEC) {
             // Unit c of rows r0, r0 + 16, ...: each thread copies what it will convert, RAWS blocks of rows ahead, and only waits for itself.
             const int c = lane & 15, r0 = warp * 2 + (lane >> 4);
-            const int nc = n0 + c * 8, kc = k0 + c * 8;     // first column of dy and x
-            const bool n_in = nc < p.N, k_in = kc < p.K;
+            const int nc = n0 + c * (16 / (int)sizeof(T)), kc = k0 + c * 8;       // first column of dy and x
+            const bool n_in = nc < p.N, n2_in = PIECES == 2 && nc + 64 < p.N, k_in = kc < p.K;
             uint8_t* raw = smem + W8_STAGES * STAGE + tid * 16;
             uint32_t e[2][4];                               // steps, of this block and the next
             const int64_t row0 = first * W8_ROWS + r0, dy_row = (int64_t)p.N * (int)sizeof(T), left0 = p.rows - row0;
@@ -130,10 +137,10 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const bool in = 16 * i < copy_left;
-                    const uint8_t* from = in && n_in ? dy_at + 16 * i * dy_row : (const uint8_t*)p.dy;
                     const int8_t* codes = in && k_in ? codes_at + 16 * i * p.K : p.codes;
-#pragma unroll
-                    for (int j = 0; j < PIECES; ++j) cp_async_zfill<16>(to + (i * PIECES + j) * (W8_LOADERS * 16), from + 16 * j, in && n_in);
+                    cp_async_zfill<16>(to + i * PIECES * (W8_LOADERS * 16), in && n_in ? dy_at + 16 * i * dy_row : (const uint8_t*)p.dy, in && n_in);
+                    if constexpr (PIECES == 2)
+                        cp_async_zfill<16>(to + (2 * i + 1) * (W8_LOADERS * 16), in && n2_in ? dy_at + 16 * i * dy_row + 256 : (const uint8_t*)p.dy, in && n2_in);
                     cp_async_zfill<8>(to + 4 * PIECES * (W8_LOADERS * 16) + i * (W8_LOADERS * 8) - tid * 8, codes, in && k_in);
                 }
                 cp_async_commit();
@@ -239,39 +246,46 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
                 if (++s == W8_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 16) {
-        // ------------------------------------------ MMA issuer ------------------------------------------
-        if (tc_elect()) {
-            uint32_t s = 0, ph = 0;
-            for (int k = 0; k < mine; ++k) {
-                const int chain = k / W8_CHAIN, start = k % W8_CHAIN == 0;
-                const uint32_t buf = (uint32_t)(chain & 1), d = tmem_base + buf * W8_T;
-                if (start && !mbar_wait(acc_empty(buf), (uint32_t)((chain >> 1) & 1) ^ 1u, abort_flag, 132, &g_w8_status)) break;
-                if (!mbar_wait(st_full(s), ph, abort_flag, 133, &g_w8_status)) break;
-                tc_fence_after();
-                const uint32_t st = base + s * STAGE;
-                const uint64_t a = w8_desc(st), b = w8_desc(st + P * W8_PART);
-#pragma unroll
-                for (int q = P - 1; q >= 0; --q)            // the smallest parts first
-#pragma unroll
-                    for (int k16 = 0; k16 < W8_ROWS / 16; ++k16)
-                        w8_mma(d, a + q * (W8_PART >> 4) + k16 * 128, b + k16 * 128, q < P - 1 || k16 > 0 || !start ? 1u : 0u);
-                tc_commit(st_empty(s));
-                if (k % W8_CHAIN == W8_CHAIN - 1 || k == mine - 1) tc_commit(acc_full(buf));
-                if (++s == W8_STAGES) { s = 0; ph ^= 1u; }
-            }
-        }
-        __syncwarp();
     } else {
-        // ------------------------------------------ accumulation ------------------------------------------
+        // ------------------------------------------ MMAs and accumulation ------------------------------------------
         const int q = warp & 3, half = (warp - 8) >> 2;     // columns 64 half .. + 63 of this lane's row
         const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
+        const int chains = (mine + W8_CHAIN - 1) / W8_CHAIN;
         float acc[64];
 #pragma unroll
         for (int j = 0; j < 64; ++j) acc[j] = 0.0f;
         bool alive = true;
-        const int chains = (mine + W8_CHAIN - 1) / W8_CHAIN;
+        uint32_t s = 0, ph = 0;
+        // one thread: the MMAs of a chain's blocks of rows
+        auto issue = [&](int chain) {
+            const uint32_t buf = (uint32_t)(chain & 1), d = tmem_base + buf * W8_T;
+            if (!mbar_wait(acc_empty(buf), (uint32_t)((chain >> 1) & 1) ^ 1u, abort_flag, 132, &g_w8_status)) return;
+            const int blocks = mine - chain * W8_CHAIN < W8_CHAIN ? mine - chain * W8_CHAIN : W8_CHAIN;
+            for (int k = 0; k < blocks; ++k) {
+                if (!mbar_wait(st_full(s), ph, abort_flag, 133, &g_w8_status)) return;
+                tc_fence_after();
+                const uint32_t st = base + s * STAGE;
+                const uint64_t a = w8_desc(st), b = w8_desc(st + P * W8_PART);
+#pragma unroll
+                for (int part = P - 1; part >= 0; --part)   // the smallest parts first
+#pragma unroll
+                    for (int k16 = 0; k16 < W8_ROWS / 16; ++k16)
+                        w8_mma(d, a + part * (W8_PART >> 4) + k16 * 128, b + k16 * 128, part < P - 1 || k16 > 0 || k > 0 ? 1u : 0u);
+                tc_commit(st_empty(s));
+                if (++s == W8_STAGES) { s = 0; ph ^= 1u; }
+            }
+            tc_commit(acc_full(buf));
+        };
+        if (warp == 8 && chains > 0) {
+            if (tc_elect()) issue(0);
+            __syncwarp();
+        }
         for (int k = 0; k < chains; ++k) {
+            // (the next chain's MMAs go first: they fill the other buffer while this one is read)
+            if (warp == 8 && k + 1 < chains) {
+                if (tc_elect()) issue(k + 1);
+                __syncwarp();
+            }
             const uint32_t buf = (uint32_t)(k & 1);
             if (!mbar_wait(acc_full(buf), (uint32_t)((k >> 1) & 1), abort_flag, 134, &g_w8_status)) { alive = false; break; }
             tc_fence_after();
@@ -293,7 +307,7 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == 8) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256) : "memory");
     }
@@ -304,7 +318,7 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
         if (warp < 8) {
             if constexpr (VEC) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) part[(warp * 2 + (lane >> 4)) * W8_T + (lane & 15) * 8 + j] = j & 1 ? sums[j / 2].y : sums[j / 2].x;
+                for (int j = 0; j < 8; ++j) part[(warp * 2 + (lane >> 4)) * W8_T + (P == 3 ? (lane & 15) * 4 + (j >> 2) * 64 + (j & 3) : (lane & 15) * 8 + j)] = j & 1 ? sums[j / 2].y : sums[j / 2].x;
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) part[warp * W8_T + 2 * lane + (j >> 1) * 64 + (j & 1)] = j & 1 ? sums[j / 2].y : sums[j / 2].x;
