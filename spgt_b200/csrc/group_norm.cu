@@ -594,7 +594,8 @@ static int gn_shape(int N, int64_t P, int C, int G, int dtype, int tensors, bool
     // Units of 96 MB of what is read: fewer launches against more of it found in L2 (64 x 106 x 106 x 128 fp32: units of 48 / 64 / 96 / 112
     // MB 188 / 179 / 178 / 190 us; 16 samples backward 94 / 100 / 74 / 83).
     const int64_t bytes = s.L * value_bytes, unit = bytes > 0 ? ((int64_t)96 << 20) / bytes : 1;
-    s.unit = (int)(unit < 1 ? 1 : unit > (N > 0 ? N : 1) ? (N > 0 ? N : 1) : unit);
+    const int samples = N > 0 ? N : 1, units = (int)(unit >= samples ? 1 : ceil_div<int64_t>(samples, unit < 1 ? 1 : unit));
+    s.unit = ceil_div(samples, units);                      // (units of nearly the same size)
     // As many tiles as blocks run at a time, so that a pass is one wave and its blocks end together; no tile of less than four rows of
     // vectors, nor less than twice the words that a block of the second pass merges.
     const int64_t rows = ceil_div<int64_t>(s.L / s.V, (int64_t)s.R * s.K), resident = (int64_t)num_sms() * (s.work > 256 ? 1 : s.V == 8 ? 2 : 4);
@@ -604,7 +605,7 @@ static int gn_shape(int N, int64_t P, int C, int G, int dtype, int tensors, bool
     if (tiles < 1) tiles = 1;
     s.iters = (int)(rows > tiles ? ceil_div(rows, tiles) : 1);
     tiles = rows > s.iters ? ceil_div<int64_t>(rows, s.iters) : 1;
-    if (tiles * (N > 0 ? N : 1) > 0x7fffffff) return SPGT_ERR_SHAPE;
+    if (tiles * samples > 0x7fffffff) return SPGT_ERR_SHAPE;
     s.tiles = (int)tiles;
     return SPGT_OK;
 }

@@ -206,38 +206,61 @@ template <class T, bool VEC> __global__ void __launch_bounds__(W8_THREADS, 1) we
             }
             cp_async_wait_all();
         } else {
-            // Any widths: columns 2 lane, 2 lane + 1 (+ 64) of rows warp, warp + 8, ...
+            // Any widths: columns 2 lane, 2 lane + 1 (+ 64) of rows warp, warp + 8, ...  Every load has an address inside its array and
+            // is zeroed afterwards where it lies outside the tile, so that no branch keeps the loads of four rows apart.
+            int ncol[4], kcol[4];                           // columns from the tile's first, inside the matrix
+            bool n_in[4], k_in[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int col = 2 * lane + (j >> 1) * 64 + (j & 1);
+                n_in[j] = n0 + col < p.N; k_in[j] = k0 + col < p.K;
+                ncol[j] = n_in[j] ? col : 0; kcol[j] = k_in[j] ? col : 0;
+            }
             for (int k = 0; k < mine; ++k) {
-                if (!mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status)) break;
-                uint8_t* stage = smem + s * STAGE;
-#pragma unroll 1
-                for (int i0 = 0; i0 < 8; i0 += 4) {
-                    float d[4][4], x[4][4];
+                float d[2][4][4];
+                uint32_t codes[2][4][4], size[2][4][4];
+                auto load = [&](int batch) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int64_t r = (first + k) * W8_ROWS + warp + 8 * (i0 + i);
+                        const int64_t r = (first + k) * W8_ROWS + warp + 8 * (4 * batch + i);
+                        const bool in = r < p.rows;
+                        const int64_t row = in ? r : 0, at = row * p.K + k0;
+                        const T* dy = (const T*)p.dy + row * p.N + n0;
+                        const int8_t* code = p.codes + at;
+                        const uint8_t* step = p.steps + (at >> 5);
+                        const int phase = (int)(at & 31);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int col = 2 * lane + (j >> 1) * 64 + (j & 1);
-                            d[i][j] = x[i][j] = 0.0f;
-                            if (r < p.rows && n0 + col < p.N) d[i][j] = to_f32(((const T*)p.dy)[r * p.N + n0 + col]);
-                            if (r < p.rows && k0 + col < p.K) {
-                                const int64_t at = r * p.K + k0 + col;
-                                x[i][j] = (float)p.codes[at] * q8_step(p.steps[at >> 5]);
-                            }
+                            d[batch][i][j] = to_f32(__ldg(dy + ncol[j]));
+                            codes[batch][i][j] = (uint32_t)(int)__ldg(code + kcol[j]);
+                            size[batch][i][j] = __ldg(step + ((phase + kcol[j]) >> 5));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (!in || !n_in[j]) d[batch][i][j] = 0.0f;
+                            if (!in || !k_in[j]) { codes[batch][i][j] = 0; size[batch][i][j] = 1; }
                         }
                     }
+                };
+                load(0);
+                if (!mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status)) break;
+                uint8_t* stage = smem + s * STAGE;
+#pragma unroll
+                for (int batch = 0; batch < 2; ++batch) {
+                    if (batch == 0) load(1);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int r = warp + 8 * (i0 + i);
+                        const int r = warp + 8 * (4 * batch + i);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {       // 64-column half
                             uint8_t* at = stage + w8_at(r, 8 * h + (lane >> 2)) + (lane & 3) * 4;
-                            float2 b = make_float2(d[i][2 * h], d[i][2 * h + 1]);
+                            float2 b = make_float2(d[batch][i][2 * h], d[batch][i][2 * h + 1]);
                             sums[h] = add2(sums[h], b);
 #pragma unroll
                             for (int q = 0; q < P; ++q, b = w8_rest(b)) *reinterpret_cast<uint32_t*>(at + q * W8_PART) = w8_upper(b);
-                            *reinterpret_cast<uint32_t*>(at + P * W8_PART) = pack_pair(make_float2(x[i][2 * h], x[i][2 * h + 1]), __nv_bfloat16{});
+                            *reinterpret_cast<uint32_t*>(at + P * W8_PART) = pack_pair(
+                                make_float2((float)(int)codes[batch][i][2 * h] * q8_step(size[batch][i][2 * h]), (float)(int)codes[batch][i][2 * h + 1] * q8_step(size[batch][i][2 * h + 1])),
+                                __nv_bfloat16{});
                         }
                     }
                 }

@@ -10,7 +10,7 @@ class Group_Norm_Act_Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, X, weight, bias, num_groups, eps, activation, activation_bits):
         X = X.contiguous()
-        Y, stats, kept = ops.group_norm(X, num_groups, weight, bias, eps, activation, compress=activation_bits == 8)
+        Y, stats, kept = ops.group_norm_forward(X, num_groups, weight, bias, eps, activation, activation_bits == 8)
         ctx.args = (num_groups, activation, X.shape, X.dtype)
         ctx.save_for_backward(weight, bias, stats, *((X,) if kept is None else (kept.codes, kept.steps)))
         return Y
@@ -34,4 +34,4 @@ def group_norm_act(X: Tensor, num_groups: int, weight: Tensor = None, bias: Tens
         raise ValueError('activation_bits must be 8 or 32')
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (X, weight, bias)):
         return Group_Norm_Act_Function.apply(X, weight, bias, num_groups, eps, activation, activation_bits)
-    return ops.group_norm(X, num_groups, weight, bias, eps, activation)[0]
+    return ops.group_norm_forward(X, num_groups, weight, bias, eps, activation, False)[0]

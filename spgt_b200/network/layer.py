@@ -156,7 +156,7 @@ class GroupNormAct(torch.nn.Module):
 
     def forward_inference(self, X: Tensor, act=None) -> Tensor:
         """Without gradients; act: an activation in place of the module's own."""
-        return ops.group_norm(X, self.num_groups, self.weight.detach(), self.bias.detach(), self.eps, self.activation if act is None else act)[0]
+        return ops.group_norm_forward(X, self.num_groups, self.weight.detach(), self.bias.detach(), self.eps, self.activation if act is None else act, False)[0]
 
 
 class ConvResBlock2D(_KernelWeights):

@@ -26,7 +26,7 @@ def act_code(name) -> int:
 
 def _stream() -> int:
     """The current stream's handle, without the Stream object that torch.cuda.current_stream() makes (5 us of a small call)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 class _device:
@@ -38,7 +38,7 @@ class _device:
         self.want, self.back = device.index, None
 
     def __enter__(self):
-        current = torch.cuda.current_device()
+        current = torch._C._cuda_getDevice()
         if self.want is not None and self.want != current:
             torch.cuda.set_device(self.want)
             self.back = current
@@ -938,14 +938,15 @@ def _norm_param(t: Optional[Tensor], name: str, C: int, device) -> Optional[int]
 
 
 def _norm_launches(N: int, sample_bytes: int) -> int:
-    """Two passes for each unit of samples (group_norm.cu: 96 MB of what both read, a sample at least)."""
-    return 0 if N * sample_bytes == 0 else -(-N // max(1, (96 << 20) // sample_bytes)) * 2
+    """Two passes for each unit of samples (group_norm.cu: up to 96 MB of what both read, a sample at least)."""
+    if N * sample_bytes == 0:
+        return 0
+    units = -(-N // max(1, (96 << 20) // sample_bytes))
+    return -(-N // -(-N // units)) * 2
 
 
-def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1.0e-5, act=None,
-               compress: bool = False):
-    """(act(group_norm(x) * weight + bias), statistics [N, num_groups, 2], x in 8 bits or None) for x [N, ..., C], channels last;
-    weight, bias [C] fp32 or None."""
+def group_norm_forward(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, act, compress: bool):
+    """(y, a buffer that begins with the statistics [N, num_groups, 2], x in 8 bits or None): group_norm without a view of the statistics."""
     code = _dtype(x, 'x')
     N, P, C = _norm_sizes(x, num_groups)
     device = x.device
@@ -957,17 +958,29 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optio
         need = lib.spgt_group_norm_workspace_bytes(N, P, C, num_groups, code)
         if need == 0:
             raise ValueError(f'unsupported sizes: {C} channels, {N} samples of {P} pixels')
-        y, stats = torch.empty_like(x), x.new_empty((N, num_groups, 2), dtype=torch.float32)
-        kept = Checkpoint8._empty(x) if compress else None
-        ws = x.new_empty(need, dtype=torch.uint8)
-        _call('spgt_group_norm_fwd', x.data_ptr(), w, b, y.data_ptr(), stats.data_ptr(), kept.codes.data_ptr() if compress else None,
-              kept.steps.data_ptr() if compress else None, N, P, C, num_groups, eps, act_code(act), code, ws.data_ptr(), need, _stream(),
-              kernels=_norm_launches(N, P * C * x.element_size()) + (compress and C % 32 != 0 and N * P > 0))
-    return y, stats, kept
+        stats_bytes = (N * num_groups * 8 + 15) // 16 * 16
+        y, buf = torch.empty_like(x), x.new_empty((stats_bytes + need + 3) // 4, dtype=torch.float32)
+        kept, codes, steps = None, None, None
+        if compress:
+            kept = Checkpoint8._empty(x)
+            codes, steps = kept.codes.data_ptr(), kept.steps.data_ptr()
+        stats = buf.data_ptr()
+        _call('spgt_group_norm_fwd', x.data_ptr(), w, b, y.data_ptr(), stats, codes, steps, N, P, C, num_groups, eps, act_code(act), code, stats + stats_bytes, need,
+              _stream(), kernels=_norm_launches(N, P * C * x.element_size()) + (compress and C % 32 != 0 and N * P > 0))
+    return y, buf, kept
+
+
+def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1.0e-5, act=None,
+               compress: bool = False):
+    """(act(group_norm(x) * weight + bias), statistics [N, num_groups, 2], x in 8 bits or None) for x [N, ..., C], channels last;
+    weight, bias [C] fp32 or None.  The statistics: mean and 1 / sqrt(variance + eps)."""
+    y, buf, kept = group_norm_forward(x, num_groups, weight, bias, eps, act, compress)
+    return y, buf[:2 * x.shape[0] * num_groups].view(x.shape[0], num_groups, 2), kept
 
 
 def group_norm_backward(grad_out: Tensor, x, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor, act=None):
-    """(dx, dweight [C], dbias [C]) of group_norm for x, the forward's input or a Checkpoint8 of it, and the forward's statistics."""
+    """(dx, dweight [C], dbias [C]) of group_norm for x, the forward's input or a Checkpoint8 of it, and the forward's statistics (or
+    the buffer that begins with them)."""
     code = _dtype(grad_out, 'grad_out')
     device = grad_out.device
     N, P, C = _norm_sizes(grad_out, num_groups)
@@ -981,13 +994,16 @@ def group_norm_backward(grad_out: Tensor, x, num_groups: int, weight: Optional[T
         x = _aligned(_same(x, 'x', grad_out.shape, device))
         values, codes, steps = x.data_ptr(), None, None
     w, b = _norm_param(weight, 'weight', C, device), _norm_param(bias, 'bias', C, device)
-    stats, grad_out = _aligned(_same(_chk(stats, 'stats'), 'stats', (N, num_groups, 2), device)), _aligned(grad_out)
+    _chk(stats, 'stats')
+    if stats.device != device or (stats.numel() < 2 * N * num_groups if stats.dim() == 1 else stats.shape != (N, num_groups, 2)):
+        raise ValueError(f'stats must be [{N}, {num_groups}, 2] on {device}, got {tuple(stats.shape)}')
+    stats, grad_out = _aligned(stats), _aligned(grad_out)
     with _device(device):
         need = lib.spgt_group_norm_bwd_workspace_bytes(N, P, C, num_groups, code)
         if need == 0:
             raise ValueError(f'unsupported sizes: {C} channels, {N} samples of {P} pixels')
         dx = torch.empty_like(grad_out)
-        dw, db = grad_out.new_empty(C, dtype=torch.float32), grad_out.new_empty(C, dtype=torch.float32)
+        dw, db = grad_out.new_empty((2, C), dtype=torch.float32).unbind(0)
         ws = grad_out.new_empty(need, dtype=torch.uint8)
         _call('spgt_group_norm_bwd', grad_out.data_ptr(), values, codes, steps, w, b, stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
               N, P, C, num_groups, act_code(act), code, ws.data_ptr(), need, _stream(),
