@@ -4,7 +4,7 @@
 // On the bf16 tensor cores, exactly: a checkpoint's value has seven significant bits and is a bf16 number as it is; dy is the sum of
 // three bf16 numbers (fp32: 8 + 8 + 8 bits, cut off, so nothing overflows), two (fp16) or one (bf16).  All products are exact in fp32.
 // The sums run over the rows, and row-major blocks of rows are what an MMA takes as MN-major operands: nothing is transposed.  Sixteen
-// warps copy blocks of 32 rows ahead and store them as bf16 parts with the 128-byte swizzle (64 columns of a row are a line); per 16 rows
+// warps copy blocks of 32 or 64 rows ahead and store them as bf16 parts with the 128-byte swizzle (64 columns of a row are a line); per 16 rows
 // and part one MMA of 128 columns of dy x up to 256 of x: so dy is converted once for all of x.
 // The accumulate step of an MMA truncates: the upper parts' sums and the others' have accumulators of their own, and after 1280 rows
 // they are added to the block's result in memory.  Error against 64 bits relative to the plain fp32 product's: below it (measured with
@@ -18,20 +18,27 @@ namespace spgt {
 
 __device__ int g_w8_status = 0;
 
-constexpr int W8_T = 128, W8_ROWS = 32, W8_THREADS = 640, W8_LOADERS = 512, W8_RAWS = 4, W8_BAR = 256;
-constexpr int W8_CHAIN = 1280 / W8_ROWS;                    // blocks of rows that an accumulator sums
-constexpr int W8_HALF = W8_ROWS * 128;                      // 64 columns of a block's rows: lines of 128 bytes
-constexpr int W8_PART = 2 * W8_HALF;                        // 128 columns
+constexpr int W8_T = 128, W8_THREADS = 640, W8_LOADERS = 512, W8_BAR = 256, W8_CHAIN = 1280;    // rows that an accumulator sums
 
 template <class T> struct W8Parts { static constexpr int N = 3; };
 template <> struct W8Parts<__half> { static constexpr int N = 2; };
 template <> struct W8Parts<__nv_bfloat16> { static constexpr int N = 1; };
-// BN: columns of x in a tile, 128 or 256.  Raw values of a block of rows per loading thread: eight columns of dy, in 16-byte pieces, and
-// BN / 128 times eight codes.
+// BN: columns of x in a tile, 128 or 256, and with it rows of a block.
 template <class T, int BN> struct W8 {
-    static constexpr int P = W8Parts<T>::N, STAGES = P == 3 ? 3 : 4, STAGE = (P + BN / W8_T) * W8_PART, PIECES = 8 * (int)sizeof(T) / 16, UNITS = BN / 128;
-    static constexpr int RAW = W8_LOADERS * (16 * PIECES + 8 * UNITS), BAR = STAGES * STAGE + W8_RAWS * RAW, SMEM = BAR + W8_BAR;
-    static constexpr int COLUMNS = (P > 1 ? 2 : 1) * BN;    // of tensor memory: the upper parts' sums, then the others'
+    static constexpr int P = W8Parts<T>::N, ROWS = BN == 256 ? 32 : 64;
+    static constexpr int HALF = ROWS * 128, PART = 2 * HALF;                   // 64 columns of a block's rows: lines of 128 bytes; 128 columns
+    static constexpr int STAGE = (P + BN / W8_T) * PART, STAGES = BN == 256 ? (P == 3 ? 3 : 4) : 5 - P;
+    // raw values of a block per loading thread: DU times eight columns of dy, in 16-byte pieces, and XU times eight codes
+    static constexpr int PIECES = 8 * (int)sizeof(T) / 16, DU = ROWS / 32, XU = ROWS * BN / (8 * W8_LOADERS);
+    static constexpr int RAW = W8_LOADERS * (16 * PIECES * DU + 8 * XU), RAWS = BN == 256 ? 4 : 5 - P;
+    static constexpr int BAR = STAGES * STAGE + RAWS * RAW, SMEM = BAR + W8_BAR, CHAIN = W8_CHAIN / ROWS;
+    static constexpr int COLUMNS = (P > 1 ? 2 : 1) * BN;                       // of tensor memory: the upper parts' sums, then the others'
+    // where unit c (of eight columns) of row r lies in a part
+    static __device__ __forceinline__ uint32_t at(int r, int c) { return (uint32_t)((c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+    // MN-major, 128-byte swizzle: 64-column blocks HALF apart (leading), groups of eight rows 1024 bytes apart (stride)
+    static __device__ __forceinline__ uint64_t desc(uint32_t smem) {
+        return (uint64_t)((smem >> 4) & 0x3fffu) | ((uint64_t)(HALF >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+    }
     static_assert(SMEM <= 227 * 1024 && 8 * (2 * STAGES + 2) <= 96, "shared memory budget");
 };
 
@@ -51,13 +58,6 @@ __device__ __forceinline__ float2 w8_rest(float2 x) {
 __device__ __forceinline__ uint32_t w8_upper(float2 x) { return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632); }
 // a 16-byte unit of bf16 from eight fp32 numbers' upper halves
 __device__ __forceinline__ uint4 w8_upper(const float2 (&b)[4]) { return make_uint4(w8_upper(b[0]), w8_upper(b[1]), w8_upper(b[2]), w8_upper(b[3])); }
-// where unit c (of eight columns) of row r lies in a part
-__device__ __forceinline__ uint32_t w8_at(int r, int c) { return (uint32_t)((c >> 3) * W8_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
-
-__device__ __forceinline__ uint64_t w8_desc(uint32_t smem) {
-    // MN-major, 128-byte swizzle: 64-column blocks W8_HALF apart (leading), groups of eight rows 1024 bytes apart (stride)
-    return (uint64_t)((smem >> 4) & 0x3fffu) | ((uint64_t)(W8_HALF >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
 // D[tmem] (+)= A B: M = 128, N = BN, K = 16, bf16 both, both MN-major, fp32 accumulators
 template <int BN> __device__ __forceinline__ void w8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(W8_T >> 4) << 24);
@@ -71,7 +71,7 @@ template <int BN> __device__ __forceinline__ void w8_mma(uint32_t d, uint64_t a,
 // VEC: N and K are multiples of eight, so eight columns of a row are in or out together and start on a boundary of their size.
 template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREADS, 1) weight_gradient8_kernel(const W8Params p) {
     using W = W8<T, BN>;
-    constexpr int P = W::P, STAGES = W::STAGES, STAGE = W::STAGE, PIECES = W::PIECES, UNITS = W::UNITS;
+    constexpr int P = W::P, STAGES = W::STAGES, STAGE = W::STAGE, PIECES = W::PIECES, DU = W::DU, XU = W::XU, RAWS = W::RAWS, ROWS = W::ROWS, HALF = W::HALF, PART = W::PART;
     extern __shared__ __align__(1024) uint8_t smem[];
     pdl_launch_next();                                      // (the second kernel waits for the end of this one)
     const uint32_t base = smem_u32(smem), bars = base + W::BAR;
@@ -86,7 +86,7 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + W::BAR + 104);
     const int tid = threadIdx.x, warp = (int)tc_uniform(tid >> 5), lane = tid & 31;
     const int tile = blockIdx.y, n0 = tile / p.kt * W8_T, k0 = tile % p.kt * BN;
-    const int64_t blocks = (p.rows + W8_ROWS - 1) / W8_ROWS, first = blocks * blockIdx.x / p.splits;
+    const int64_t blocks = (p.rows + ROWS - 1) / ROWS, first = blocks * blockIdx.x / p.splits;
     const int mine = (int)(blocks * (blockIdx.x + 1) / p.splits - first);
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(st_full(s), W8_LOADERS / 32); mbar_init(st_empty(s), 1); }
@@ -114,73 +114,81 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
             if (++s == STAGES) { s = 0; ph ^= 1u; }
         };
         if constexpr (VEC) {
-            // dy: unit c of row r; fp32: columns 4 c .. + 3 and 64 + 4 c .. + 3, so that the lanes' 16-byte copies are next to each other.
-            // x: unit kc of rows kr, kr + 16.  Each thread copies what it will convert, W8_RAWS blocks ahead, and only waits for itself.
-            const int c = tid & 15, r = tid >> 4, kc = UNITS == 2 ? tid & 31 : c, kr = UNITS == 2 ? tid >> 5 : r;
+            // dy: unit c of rows r, r + 32; fp32: columns 4 c .. + 3 and 64 + 4 c .. + 3, so that the lanes' 16-byte copies are next to each
+            // other.  x: unit kc of rows kr, kr + KSTEP.  Each thread copies what it will convert, RAWS blocks ahead, and only waits for itself.
+            constexpr int KSTEP = ROWS / XU;
+            const int c = tid & 15, r = tid >> 4, kc = BN == 256 ? tid & 31 : c, kr = BN == 256 ? tid >> 5 : r;
             const int nc = n0 + c * (16 / (int)sizeof(T));
             const bool n_in = nc < p.N, n2_in = PIECES == 2 && nc + 64 < p.N, k_in = k0 + kc * 8 < p.K;
             uint8_t* raw = smem + STAGES * STAGE + tid * 16;
-            uint8_t* raw_codes = smem + STAGES * STAGE + PIECES * (W8_LOADERS * 16) + tid * 8;
-            const int64_t end = (first + mine) * W8_ROWS < p.rows ? (first + mine) * W8_ROWS : p.rows, dy_row = (int64_t)p.N * (int)sizeof(T);
-            int64_t row = first * W8_ROWS;                  // of the block to copy
+            uint8_t* raw_codes = smem + STAGES * STAGE + DU * PIECES * (W8_LOADERS * 16) + tid * 8;
+            const int64_t end = (first + mine) * ROWS < p.rows ? (first + mine) * ROWS : p.rows, dy_row = (int64_t)p.N * (int)sizeof(T);
+            int64_t row = first * ROWS;                     // of the block to copy
             const uint8_t* dy_at = (const uint8_t*)p.dy + (row + r) * dy_row + (int64_t)nc * (int)sizeof(T);
             int64_t at = (row + kr) * p.K + k0 + kc * 8;    // value of x
             int slot_in = 0, slot_out = 0;
             // the steps are loaded with the copies and held until their block's turn
-            uint32_t e[W8_RAWS][UNITS];
-            auto copy = [&](uint32_t (&step)[UNITS]) {
+            uint32_t e[RAWS][XU];
+            auto copy = [&](uint32_t (&step)[XU]) {
                 uint8_t* to = raw + slot_in * W::RAW;
-                const bool in = row + r < end;
-                cp_async_zfill<16>(to, in && n_in ? dy_at : (const uint8_t*)p.dy, in && n_in);
-                if constexpr (PIECES == 2) cp_async_zfill<16>(to + W8_LOADERS * 16, in && n2_in ? dy_at + 256 : (const uint8_t*)p.dy, in && n2_in);
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u) {
-                    const bool there = k_in && row + kr + 16 * u < end;
-                    const int64_t from = there ? at + 16 * u * (int64_t)p.K : 0;
+                for (int u = 0; u < DU; ++u) {
+                    const bool in = row + r + 32 * u < end;
+                    const uint8_t* from = dy_at + 32 * u * dy_row;
+                    cp_async_zfill<16>(to + u * PIECES * (W8_LOADERS * 16), in && n_in ? from : (const uint8_t*)p.dy, in && n_in);
+                    if constexpr (PIECES == 2) cp_async_zfill<16>(to + (2 * u + 1) * (W8_LOADERS * 16), in && n2_in ? from + 256 : (const uint8_t*)p.dy, in && n2_in);
+                }
+#pragma unroll
+                for (int u = 0; u < XU; ++u) {
+                    const bool there = k_in && row + kr + KSTEP * u < end;
+                    const int64_t from = there ? at + KSTEP * u * (int64_t)p.K : 0;
                     cp_async_zfill<8>(raw_codes + slot_in * W::RAW + u * (W8_LOADERS * 8), p.codes + from, there);
                     step[u] = there ? __ldg(p.steps + (from >> 5)) : 1u;
                 }
                 cp_async_commit();
-                row += W8_ROWS; dy_at += W8_ROWS * dy_row; at += W8_ROWS * (int64_t)p.K;
-                slot_in = slot_in == W8_RAWS - 1 ? 0 : slot_in + 1;
+                row += ROWS; dy_at += ROWS * dy_row; at += ROWS * (int64_t)p.K;
+                slot_in = slot_in == RAWS - 1 ? 0 : slot_in + 1;
             };
             if (mine > 0) {
 #pragma unroll
-                for (int k = 0; k < W8_RAWS; ++k) copy(e[k]);
+                for (int k = 0; k < RAWS; ++k) copy(e[k]);
             }
-            auto step = [&](uint32_t (&size)[UNITS]) {
-                cp_async_wait<W8_RAWS - 1>();
+            auto step = [&](uint32_t (&size)[XU]) {
+                cp_async_wait<RAWS - 1>();
                 if (!__all_sync(0xffffffffu, mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status))) return false;
                 uint8_t* stage = smem + s * STAGE;
                 const uint8_t* from = raw + slot_out * W::RAW;
-                float2 b[4];
-                if constexpr (PIECES == 2) {
-                    float2 h[2];
-                    unpack_pairs(*reinterpret_cast<const uint4*>(from), h, 0.0f);
-                    b[0] = h[0]; b[1] = h[1];
-                    unpack_pairs(*reinterpret_cast<const uint4*>(from + W8_LOADERS * 16), h, 0.0f);
-                    b[2] = h[0]; b[3] = h[1];
-                } else {
-                    unpack_pairs(*reinterpret_cast<const uint4*>(from), b, T{});
-                }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sums[j] = add2(sums[j], b[j]);
-                const uint32_t to = PIECES == 2 ? w8_at(r, c >> 1) + (c & 1) * 8 : w8_at(r, c);
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
+                for (int u = 0; u < DU; ++u) {
+                    float2 b[4];
                     if constexpr (PIECES == 2) {
-                        *reinterpret_cast<uint2*>(stage + q * W8_PART + to) = make_uint2(w8_upper(b[0]), w8_upper(b[1]));
-                        *reinterpret_cast<uint2*>(stage + q * W8_PART + W8_HALF + to) = make_uint2(w8_upper(b[2]), w8_upper(b[3]));
+                        float2 h[2];
+                        unpack_pairs(*reinterpret_cast<const uint4*>(from + 2 * u * (W8_LOADERS * 16)), h, 0.0f);
+                        b[0] = h[0]; b[1] = h[1];
+                        unpack_pairs(*reinterpret_cast<const uint4*>(from + (2 * u + 1) * (W8_LOADERS * 16)), h, 0.0f);
+                        b[2] = h[0]; b[3] = h[1];
                     } else {
-                        *reinterpret_cast<uint4*>(stage + q * W8_PART + to) = w8_upper(b);
+                        unpack_pairs(*reinterpret_cast<const uint4*>(from + u * (W8_LOADERS * 16)), b, T{});
                     }
-                    if (q + 1 < P) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) b[j] = w8_rest(b[j]);
+                    for (int j = 0; j < 4; ++j) sums[j] = add2(sums[j], b[j]);
+                    const uint32_t to = PIECES == 2 ? W::at(r + 32 * u, c >> 1) + (c & 1) * 8 : W::at(r + 32 * u, c);
+#pragma unroll
+                    for (int q = 0; q < P; ++q) {
+                        if constexpr (PIECES == 2) {
+                            *reinterpret_cast<uint2*>(stage + q * PART + to) = make_uint2(w8_upper(b[0]), w8_upper(b[1]));
+                            *reinterpret_cast<uint2*>(stage + q * PART + HALF + to) = make_uint2(w8_upper(b[2]), w8_upper(b[3]));
+                        } else {
+                            *reinterpret_cast<uint4*>(stage + q * PART + to) = w8_upper(b);
+                        }
+                        if (q + 1 < P) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) b[j] = w8_rest(b[j]);
+                        }
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u) {
+                for (int u = 0; u < XU; ++u) {
                     const uint2 q = *reinterpret_cast<const uint2*>(raw_codes + slot_out * W::RAW + u * (W8_LOADERS * 8));
                     const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
                     const float2 scale = pair(q8_step(size[u]));
@@ -191,30 +199,31 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
                         const float2 code = make_float2(__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + 2 * (j & 1))), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7541 + 2 * (j & 1))));
                         y[j] = mul2(add2(code, pair(-8388736.0f)), scale);
                     }
-                    *reinterpret_cast<uint4*>(stage + P * W8_PART + w8_at(kr + 16 * u, kc)) = pack_pairs(y, __nv_bfloat16{});
+                    *reinterpret_cast<uint4*>(stage + P * PART + W::at(kr + KSTEP * u, kc)) = pack_pairs(y, __nv_bfloat16{});
                 }
-                slot_out = slot_out == W8_RAWS - 1 ? 0 : slot_out + 1;
+                slot_out = slot_out == RAWS - 1 ? 0 : slot_out + 1;
                 copy(size);
                 stored();
                 return true;
             };
             bool alive = true;
-            for (int k = 0; k < mine && alive; k += W8_RAWS) {
+            for (int k = 0; k < mine && alive; k += RAWS) {
 #pragma unroll
-                for (int j = 0; j < W8_RAWS; ++j)
+                for (int j = 0; j < RAWS; ++j)
                     if (alive && k + j < mine) alive = step(e[j]);
             }
             cp_async_wait_all();
         } else {
-            // Any widths: columns 2 lane, 2 lane + 1 (+ 64, ...) of rows warp, warp + 16.  Every load has an address inside its array and is
+            // Any widths: columns 2 lane, 2 lane + 1 (+ 64, ...) of rows warp, warp + 16, ...  Every load has an address inside its array and is
             // zeroed afterwards where it lies outside the tile, so that no branch keeps the loads apart.
             constexpr int NJ = 4, KJ = BN / 32;
-            for (int k = 0; k < mine; ++k) {
+            for (int part = 0; part < mine * (ROWS / 32); ++part) {
+                const int k = part / (ROWS / 32), r0 = warp + part % (ROWS / 32) * 32;       // two rows of 32 at a time
                 float d[2][NJ];
                 uint32_t codes[2][KJ], size[2][KJ];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int64_t r = (first + k) * W8_ROWS + warp + 16 * i;
+                    const int64_t r = (first + k) * ROWS + r0 + 16 * i;
                     const bool in = r < p.rows;
                     const int64_t row = in ? r : 0, at = row * p.K + k0;
                     const T* dy = (const T*)p.dy + row * p.N + n0;
@@ -235,30 +244,30 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
                         if (col >= k_left) { codes[i][j] = 0; size[i][j] = 1; }
                     }
                 }
-                if (!__all_sync(0xffffffffu, mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status))) break;
+                if (r0 < 32 && !__all_sync(0xffffffffu, mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status))) break;
                 uint8_t* stage = smem + s * STAGE;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int r = warp + 16 * i;
-                    const uint32_t to = w8_at(r, lane >> 2) + (lane & 3) * 4;
+                    const int r = r0 + 16 * i;
+                    const uint32_t to = W::at(r, lane >> 2) + (lane & 3) * 4;
 #pragma unroll
                     for (int h = 0; h < NJ / 2; ++h) {      // 64 columns each
                         float2 b = make_float2(d[i][2 * h], d[i][2 * h + 1]);
                         sums[h] = add2(sums[h], b);
 #pragma unroll
-                        for (int q = 0; q < P; ++q, b = w8_rest(b)) *reinterpret_cast<uint32_t*>(stage + q * W8_PART + h * W8_HALF + to) = w8_upper(b);
+                        for (int q = 0; q < P; ++q, b = w8_rest(b)) *reinterpret_cast<uint32_t*>(stage + q * PART + h * HALF + to) = w8_upper(b);
                     }
 #pragma unroll
                     for (int h = 0; h < KJ / 2; ++h)
-                        *reinterpret_cast<uint32_t*>(stage + P * W8_PART + h * W8_HALF + to) = pack_pair(
+                        *reinterpret_cast<uint32_t*>(stage + P * PART + h * HALF + to) = pack_pair(
                             make_float2((float)(int)codes[i][2 * h] * q8_step(size[i][2 * h]), (float)(int)codes[i][2 * h + 1] * q8_step(size[i][2 * h + 1])), __nv_bfloat16{});
                 }
-                stored();
+                if (r0 + 32 >= ROWS) stored();
             }
         }
     } else {
         // ------------------------------------------ MMAs and results ------------------------------------------
-        const int chains = mine > 0 ? (mine + W8_CHAIN - 1) / W8_CHAIN : 0;
+        const int chains = mine > 0 ? (mine + W::CHAIN - 1) / W::CHAIN : 0;
         uint32_t s = 0, ph = 0;
         float* out = p.partial + (((int64_t)blockIdx.x * gridDim.y + tile) * W8_T + (warp - 16) * 32 + lane) * BN;
         const uint32_t row = tmem_base + ((uint32_t)((warp - 16) * 32) << 16);
@@ -266,17 +275,17 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
         auto issue = [&](int chain) {
             if (!mbar_wait(acc_empty, (uint32_t)(chain & 1) ^ 1u, abort_flag, 132, &g_w8_status)) return;
             tc_fence_after();
-            const int n = mine - chain * W8_CHAIN < W8_CHAIN ? mine - chain * W8_CHAIN : W8_CHAIN;
+            const int n = mine - chain * W::CHAIN < W::CHAIN ? mine - chain * W::CHAIN : W::CHAIN;
             for (int k = 0; k < n; ++k) {
                 if (!mbar_wait(st_full(s), ph, abort_flag, 133, &g_w8_status)) return;
                 tc_fence_after();
                 const uint32_t st = base + s * STAGE;
-                const uint64_t a = w8_desc(st), b = w8_desc(st + P * W8_PART);
+                const uint64_t a = W::desc(st), b = W::desc(st + P * PART);
 #pragma unroll
                 for (int part = P - 1; part >= 0; --part)   // the smallest parts first
 #pragma unroll
-                    for (int k16 = 0; k16 < W8_ROWS / 16; ++k16)
-                        w8_mma<BN>(tmem_base + (part ? BN : 0), a + part * (W8_PART >> 4) + k16 * 128, b + k16 * 128,
+                    for (int k16 = 0; k16 < ROWS / 16; ++k16)
+                        w8_mma<BN>(tmem_base + (part ? BN : 0), a + part * (PART >> 4) + k16 * 128, b + k16 * 128,
                                    k > 0 || k16 > 0 || (part > 0 && part < P - 1) ? 1u : 0u);
                 tc_commit(st_empty(s));
                 if (++s == STAGES) { s = 0; ph ^= 1u; }
@@ -386,10 +395,10 @@ template <int BN> __global__ void __launch_bounds__(256) weight_gradient8_reduce
 
 // Tiles of 128 columns of x where that is all there are, of 256 otherwise.
 static inline int w8_width(int K) { return K <= W8_T ? W8_T : 2 * W8_T; }
-// Blocks that share the rows: one wave over the SMs, at least four blocks of rows each
+// Blocks that share the rows: one wave over the SMs, at least 128 rows each
 static int w8_splits(int N, int K, int64_t rows) {
     const int tiles = ceil_div(N, W8_T) * ceil_div(K, w8_width(K)), most = num_sms() / tiles < 1 ? 1 : num_sms() / tiles;
-    const int64_t want = ceil_div<int64_t>(rows, W8_ROWS * 4);
+    const int64_t want = ceil_div<int64_t>(rows, 128);
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
