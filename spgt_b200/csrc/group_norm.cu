@@ -265,7 +265,7 @@ template <class F, class B> __device__ __forceinline__ void gn_words(const GnPar
             if (pass == 0 || s.tiles > batch) {
 #pragma unroll
                 for (int i = 0; i < GN_HELD; ++i)
-                    if (from + i * s.lanes < tiles) v[i] = __ldca(at + (int64_t)(from + i * s.lanes) * s.G);
+                    if (from + i * s.lanes < tiles) v[i] = __ldcg(at + (int64_t)(from + i * s.lanes) * s.G);
             }
 #pragma unroll
             for (int i = 0; i < GN_HELD; ++i)
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(512) gn_params_kernel(const float2* chan, int6
     float2 sum = make_float2(0.0f, 0.0f);
     if (c < C)
 #pragma unroll 8
-        for (int64_t k = (blockIdx.x & 7) * 16 + w; k < rows; k += 128) { const float2 v = __ldca(chan + k * C + c); sum.x += v.x; sum.y += v.y; }
+        for (int64_t k = (blockIdx.x & 7) * 16 + w; k < rows; k += 128) { const float2 v = __ldcg(chan + k * C + c); sum.x += v.x; sum.y += v.y; }
     part[w][lane] = sum;
     __syncthreads();
     if (w == 0) {

@@ -366,7 +366,7 @@ template <int BN> __global__ void __launch_bounds__(256) weight_gradient8_reduce
         if (in)
 #pragma unroll 8
             for (int k = g; k < p.splits; k += 8) {
-                const float4 v = __ldca(src + (int64_t)k * tiles * (W8_T * BN / 4));
+                const float4 v = __ldcg(src + (int64_t)k * tiles * (W8_T * BN / 4));
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
         part[g][lane] = s;
@@ -383,7 +383,7 @@ template <int BN> __global__ void __launch_bounds__(256) weight_gradient8_reduce
         const int c = (blockIdx.x - c_blocks) * 32 + lane;  // (whole tiles of columns)
         float s = 0.0f;
 #pragma unroll 8
-        for (int k = g; k < p.splits; k += 8) s += __ldca(p.colpart + (int64_t)k * (tiles / p.kt) * W8_T + c);
+        for (int k = g; k < p.splits; k += 8) s += __ldcg(p.colpart + (int64_t)k * (tiles / p.kt) * W8_T + c);
         part[g][lane].x = s;
         __syncthreads();
         if (g || c >= p.N) return;

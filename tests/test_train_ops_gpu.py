@@ -288,6 +288,46 @@ def test_unaligned_views_and_empty(dtype):
         assert dx.shape == shape and not dw.any() and not db.any()
 
 
+@pytest.mark.parametrize('N,P,C,G', [(3, 35, 7, 1), (5, 900, 64, 8)])
+def test_group_norm_in_place(N, P, C, G):
+    """The C entry point takes y = x, without and with a checkpoint of x."""
+    from spgt_b200._lib import lib
+    from spgt_b200 import ops
+    x = _rand(N, P, C, seed=1)
+    want, stats, kept = ops.group_norm(x, G, None, None, 1e-5, 'silu', compress=True)
+    need = lib.spgt_group_norm_workspace_bytes(N, P, C, G, 0)
+    for compress in (False, True):
+        y, s = x.clone(), torch.empty_like(stats)
+        codes, steps = torch.empty_like(kept.codes), torch.empty_like(kept.steps)
+        ws = torch.empty(need, dtype=torch.uint8, device='cuda')
+        rc = lib.spgt_group_norm_fwd(y.data_ptr(), None, None, y.data_ptr(), s.data_ptr(), codes.data_ptr() if compress else None, steps.data_ptr() if compress else None,
+                                     N, P, C, G, 1e-5, 2, 0, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(y, want) and torch.equal(s, stats)
+        assert not compress or (torch.equal(codes, kept.codes) and torch.equal(steps, kept.steps))
+
+
+def test_group_norm_several_units():
+    """More samples than one unit holds in either pass: as sample by sample."""
+    from spgt_b200 import ops
+    N, P, C, G = 9, 180 * 180, 128, 4                          # 16.6 MB a sample
+    x, dy = _rand(N, P, C, seed=1, mean=0.3), _rand(N, P, C, seed=2)
+    w, b = _rand(C, seed=3, mean=1.0, scale=0.2), _rand(C, seed=4)
+    y, stats, kept = ops.group_norm(x, G, w, b, 1e-5, 'silu', compress=True)
+    dx, dw, db = ops.group_norm_backward(dy, x, G, w, b, stats, 'silu')
+    dx8, dw8, db8 = ops.group_norm_backward(dy, kept, G, w, b, stats, 'silu')
+    sums = [torch.zeros(C, device='cuda', dtype=torch.float64) for _ in range(4)]
+    for n in range(N):
+        want = _norm64(x[n:n + 1], G, w, b, 1e-5, 'silu', dy[n:n + 1])
+        _within(y[n:n + 1], *want['y'])
+        _within(dx[n:n + 1], *want['dx'])
+        want8 = _norm64(x[n:n + 1], G, w, b, 1e-5, 'silu', dy[n:n + 1], _kept64(x[n:n + 1]))
+        _within(dx8[n:n + 1], *want8['dx'])
+        for s, v in zip(sums, (want['dw'][0], want['db'][0], want8['dw'][0], want8['db'][0])):
+            s += v
+    for got, want in zip((dw, db, dw8, db8), sums):
+        assert float((got.double() - want).norm() / want.norm()) < 2e-6
+
+
 def test_group_norm_in_place_buffers_are_kept():
     """Nothing is written behind the outputs, whatever part of a vector they end in."""
     from spgt_b200._lib import lib
@@ -312,16 +352,18 @@ def test_group_norm_in_place_buffers_are_kept():
 # ---------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('rows,N,K', [(1, 1, 1), (7, 8, 16), (63, 32, 130), (65, 1, 128), (1849, 128, 136), (1849, 256, 128), (2809, 128, 256),
-                                      (1000, 34, 42), (130, 300, 520), (4096, 33, 31), (20000, 128, 256), (517, 129, 257)])
+                                      (1000, 34, 42), (130, 300, 520), (4096, 33, 31), (20000, 128, 256), (517, 129, 257), (200000, 8, 16), (190001, 5, 130)])
 def test_weight_gradient8(dtype, rows, N, K):
     from spgt_b200 import ops
     x, dy = _rand(rows, K, seed=1, dtype=dtype, mean=0.5), _rand(rows, N, seed=2, dtype=dtype)
     kept = ops.compress8(x)
     dw, db = ops.weight_gradient8(dy, kept)
     v, d = _kept64(x), dy.double()
-    # products are exact in fp32; pieces of at most 256 rows are summed with at most 64 U each, the pieces in chains of at most 64
-    _within(dw, d.t() @ v, 128 * U * (d.abs().t() @ v.abs()) + 1e-37)
-    _within(db, d.sum(0), 128 * U * d.abs().sum(0))
+    # products are exact in fp32; an accumulator takes at most 80 additions that truncate (2 U each) before its sum moves on, and the
+    # sums of fewer than 64 pieces are added up in chains of at most 19
+    _within(dw, d.t() @ v, 192 * U * (d.abs().t() @ v.abs()) + 1e-37)
+    # a thread adds up at most rows / (148 * 16) values in a row, at most 64 of them are added in order, and at most 19 blocks' results
+    _within(db, d.sum(0), (192 + rows / 2000) * U * d.abs().sum(0))
     again = ops.weight_gradient8(dy, kept, column_sums=False)
     assert torch.equal(again[0], dw) and again[1] is None
 
