@@ -42,6 +42,7 @@ struct GnParams {
     float *dw, *db;
     float eps;
     int act, first;             // first: sample of the unit
+    bool last;                  // the launch that adds up dw and db
 };
 
 // Where a block's tile lies.
@@ -498,6 +499,34 @@ __device__ __forceinline__ float2 gn_bwd_merge(const GnParams& p, const GnTask& 
     return make_float2(lanes_sum(c1, s.lanes) / total, lanes_sum(c2, s.lanes) / total);
 }
 
+// dw and db from all tiles' sums [rows][C], by the blocks of the last launch once they have written their tile: two channels a block, a
+// share of the rows to each thread, in a fixed order.  (Backward of 16 x 106 x 106 x 128 from a checkpoint with 1 / 2 / 4 / 8 channels a
+// block 69.5 / 70.9 / 75.0 / 82.5 us, of 8 x 211 x 211 x 44 bf16 49.5 / 46.1 / 46.4 / 46.8; in a launch of its own 72.4 and 49.0.)
+constexpr int GN_PARAM_COLS = 2;
+
+__device__ __forceinline__ void gn_params(const GnParams& p, float2* part) {
+    const GnShape& s = p.s;
+    const int lane = threadIdx.x & 31, shares = s.work / GN_PARAM_COLS;
+    const int64_t rows = (int64_t)s.N * s.tiles;
+    for (int c0 = blockIdx.x * GN_PARAM_COLS; c0 < s.C; c0 += gridDim.x * GN_PARAM_COLS) {
+        const int c = c0 + (lane & (GN_PARAM_COLS - 1));
+        float2 sum = pair(0.0f);
+        if (c < s.C)
+#pragma unroll 4
+            for (int64_t k = threadIdx.x / GN_PARAM_COLS; k < rows; k += shares) sum = add2(sum, __ldcg(p.chan + k * s.C + c));
+#pragma unroll
+        for (int o = GN_PARAM_COLS; o < 32; o <<= 1) sum = add2(sum, make_float2(__shfl_xor_sync(0xffffffffu, sum.x, o), __shfl_xor_sync(0xffffffffu, sum.y, o)));
+        __syncthreads();
+        if (lane < GN_PARAM_COLS) part[(threadIdx.x >> 5) * GN_PARAM_COLS + lane] = sum;
+        __syncthreads();
+        if (threadIdx.x < GN_PARAM_COLS && c < s.C) {
+            for (int k = 1; k < s.work / 32; ++k) sum = add2(sum, part[k * GN_PARAM_COLS + lane]);
+            if (p.db) p.db[c] = sum.x;
+            if (p.dw) p.dw[c] = sum.y;
+        }
+    }
+}
+
 template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_MAX_WORK) gn_bwd_apply_kernel(const GnParams p) {
     constexpr int V = Pack<T>::N, S = JOINT ? 1 : V / 2;
     extern __shared__ float2 s_group[];
@@ -546,33 +575,7 @@ template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_
             __stcs(reinterpret_cast<uint4*>((T*)p.out + t.base + (int64_t)j * V), pack_pairs(d, T{}));
         });
     });
-}
-
-// dw and db from the tiles' sums [rows][C]: a cluster of eight blocks takes 32 channels, its blocks and their warps a share of the rows
-// each; the first block adds the shares up, in order.
-__global__ void __launch_bounds__(512) gn_params_kernel(const float2* chan, int64_t rows, int C, float* dw, float* db) {
-    __shared__ float2 part[16][32];
-    __shared__ float share[2][32];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x / 8 * 32 + lane;
-    pdl_launch_next();
-    pdl_wait();
-    float2 sum = make_float2(0.0f, 0.0f);
-    if (c < C)
-#pragma unroll 8
-        for (int64_t k = (blockIdx.x & 7) * 16 + w; k < rows; k += 128) { const float2 v = __ldcg(chan + k * C + c); sum.x += v.x; sum.y += v.y; }
-    part[w][lane] = sum;
-    __syncthreads();
-    if (w == 0) {
-        for (int k = 1; k < 16; ++k) { const float2 v = part[k][lane]; sum.x += v.x; sum.y += v.y; }
-        share[0][lane] = sum.x; share[1][lane] = sum.y;
-    }
-    cluster_sync_all();
-    if ((blockIdx.x & 7) == 0 && w == 0) {
-        for (int k = 1; k < 8; ++k) { sum.x += ld_dsmem_f32(&share[0][lane], k); sum.y += ld_dsmem_f32(&share[1][lane], k); }
-        if (c < C && db) db[c] = sum.x;
-        if (c < C && dw) dw[c] = sum.y;
-    }
-    cluster_sync_all();                                     // (the others' shared memory is read until here)
+    if (p.last) gn_params(p, s_group);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------------
@@ -687,10 +690,11 @@ extern "C" int spgt_group_norm_bwd(const void* dy, const void* x, const int8_t* 
     p.chan = p.words + (int64_t)N * s.tiles * G;
     const bool joint = s.cg % s.V == 0;
     ChainScope chain;
-    const int e = with_type(dtype, [&](auto zero) {
+    return with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
-        const size_t sums = (size_t)s.R * s.K * s.V * sizeof(float2), groups = (size_t)G * sizeof(float2);
+        const size_t sums = (size_t)s.R * s.K * s.V * sizeof(float2), groups = (size_t)(G > s.work / 4 ? G : s.work / 4) * sizeof(float2);
         for (int n = 0; n < N; n += s.unit) {
+            p.last = n + s.unit >= N && (dw || db);
             int e = joint ? (codes ? gn_launch<gn_bwd_sums_kernel<T, true, true>>(p, n, sums, st) : gn_launch<gn_bwd_sums_kernel<T, true, false>>(p, n, sums, st))
                           : (codes ? gn_launch<gn_bwd_sums_kernel<T, false, true>>(p, n, sums, st) : gn_launch<gn_bwd_sums_kernel<T, false, false>>(p, n, sums, st));
             if (e) return e;
@@ -700,18 +704,4 @@ extern "C" int spgt_group_norm_bwd(const void* dy, const void* x, const int8_t* 
         }
         return (int)SPGT_OK;
     });
-    if (e || !(dw || db)) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ceil_div(C, 32) * 8); cfg.blockDim = dim3(512); cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 8; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
-    if (const cudaError_t err = cudaLaunchKernelEx(&cfg, gn_params_kernel, (const float2*)p.chan, (int64_t)N * s.tiles, C, dw, db)) {
-        g_last_cuda_error = (int)err; (void)cudaGetLastError();
-        return SPGT_ERR_LAUNCH;
-    }
-    return SPGT_OK;
 }

@@ -6,6 +6,7 @@ torch.empty on the input's device and launches on torch's current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -937,6 +938,15 @@ def _norm_param(t: Optional[Tensor], name: str, C: int, device) -> Optional[int]
     return t.data_ptr()
 
 
+@functools.lru_cache(maxsize=1024)
+def _norm_plan(N: int, P: int, C: int, G: int, code: int, device: int) -> Tuple[int, int, int]:
+    """(bytes of the statistics, rounded up, and of both ways' workspaces); the sizes go by the device's number of SMs."""
+    need, need_bwd = lib.spgt_group_norm_workspace_bytes(N, P, C, G, code), lib.spgt_group_norm_bwd_workspace_bytes(N, P, C, G, code)
+    if need == 0 or need_bwd == 0:
+        raise ValueError(f'unsupported sizes: {C} channels, {N} samples of {P} pixels')
+    return (N * G * 8 + 15) // 16 * 16, need, need_bwd
+
+
 def _norm_launches(N: int, sample_bytes: int) -> int:
     """Two passes for each unit of samples (group_norm.cu: up to 96 MB of what both read, a sample at least)."""
     if N * sample_bytes == 0:
@@ -955,10 +965,7 @@ def group_norm_forward(x: Tensor, num_groups: int, weight: Optional[Tensor], bia
         raise ValueError('eps must not be negative')
     x = _aligned(x)
     with _device(device):
-        need = lib.spgt_group_norm_workspace_bytes(N, P, C, num_groups, code)
-        if need == 0:
-            raise ValueError(f'unsupported sizes: {C} channels, {N} samples of {P} pixels')
-        stats_bytes = (N * num_groups * 8 + 15) // 16 * 16
+        stats_bytes, need, _ = _norm_plan(N, P, C, num_groups, code, device.index)
         y, buf = torch.empty_like(x), x.new_empty((stats_bytes + need + 3) // 4, dtype=torch.float32)
         kept, codes, steps = None, None, None
         if compress:
@@ -999,13 +1006,11 @@ def group_norm_backward(grad_out: Tensor, x, num_groups: int, weight: Optional[T
         raise ValueError(f'stats must be [{N}, {num_groups}, 2] on {device}, got {tuple(stats.shape)}')
     stats, grad_out = _aligned(stats), _aligned(grad_out)
     with _device(device):
-        need = lib.spgt_group_norm_bwd_workspace_bytes(N, P, C, num_groups, code)
-        if need == 0:
-            raise ValueError(f'unsupported sizes: {C} channels, {N} samples of {P} pixels')
+        need = _norm_plan(N, P, C, num_groups, code, device.index)[2]
         dx = torch.empty_like(grad_out)
-        dw, db = grad_out.new_empty((2, C), dtype=torch.float32).unbind(0)
+        dw, db = grad_out.new_empty(C, dtype=torch.float32), grad_out.new_empty(C, dtype=torch.float32)
         ws = grad_out.new_empty(need, dtype=torch.uint8)
         _call('spgt_group_norm_bwd', grad_out.data_ptr(), values, codes, steps, w, b, stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
               N, P, C, num_groups, act_code(act), code, ws.data_ptr(), need, _stream(),
-              kernels=_norm_launches(N, P * C * dx.element_size() * 2 if codes is None else P * C * (dx.element_size() + 1)) + (N * P > 0))
+              kernels=_norm_launches(N, P * C * dx.element_size() * 2 if codes is None else P * C * (dx.element_size() + 1)))
     return dx, dw, db
