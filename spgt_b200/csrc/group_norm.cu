@@ -14,6 +14,12 @@
 // Each way is a pass for the sums, which leaves a word per group and tile, and a pass for the results, whose blocks merge their
 // sample's words themselves.  Both read x, so they take turns over units of samples that stay in L2 in between: the first pass asks L2
 // to keep what it reads, the second to let go of what it reads and writes.  Launches are chained (common.cuh), which hides their gaps.
+// Measured, in a graph: 64 x 106 x 106 x 128 fp32 177 us (reading x and writing y once takes 112 at the measured copy rate; part of the
+// second read comes from memory, and a unit's passes each start and drain), 8 x 211 x 211 x 42 bf16 24.8 (9.1; two waves' latencies), 43 x
+// 43 x 128 fp32 8.0 (two launches); backward of 4 x 71 x 71 x 128 fp32 19.4 (4.7), of 16 x 106 x 106 x 128 fp32 from a
+// checkpoint 70.6 (32), of 8 x 211 x 211 x 44 bf16 from one 46.4 (12).
+// One launch in which a cluster of 8 or 16 blocks shares a sample and meets in the middle is no faster: 178 to 191 us for the first,
+// 36.6, 9.5, and 21 to 27, 110, 67 backward.
 #include "lowp.cuh"
 
 namespace spgt {
@@ -600,7 +606,8 @@ static int gn_shape(int N, int64_t P, int C, int G, int dtype, int tensors, bool
     const int samples = N > 0 ? N : 1, units = (int)(unit >= samples ? 1 : ceil_div<int64_t>(samples, unit < 1 ? 1 : unit));
     s.unit = ceil_div(samples, units);                      // (units of nearly the same size)
     // As many tiles as blocks run at a time, so that a pass is one wave and its blocks end together; no tile of less than four rows of
-    // vectors, nor less than twice the words that a block of the second pass merges.
+    // vectors, nor less than twice the words that a block of the second pass merges.  Vectors of eight values take more registers and
+    // more merging per block: two blocks to an SM (8 x 211 x 211 x 42 bf16 with 2 / 3 / 4 / 6: 24.1 / 26.4 / 25.4 / 28.5 us).
     const int64_t rows = ceil_div<int64_t>(s.L / s.V, (int64_t)s.R * s.K), resident = (int64_t)num_sms() * (s.work > 256 ? 1 : s.V == 8 ? 2 : 4);
     int64_t tiles = resident / s.unit;
     while (tiles > 1 && tiles * tiles * 16 * G > bytes) tiles = tiles * 7 / 8;
@@ -692,7 +699,7 @@ extern "C" int spgt_group_norm_bwd(const void* dy, const void* x, const int8_t* 
     ChainScope chain;
     return with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
-        const size_t sums = (size_t)s.R * s.K * s.V * sizeof(float2), groups = (size_t)(G > s.work / 4 ? G : s.work / 4) * sizeof(float2);
+        const size_t sums = (size_t)s.R * s.K * s.V * sizeof(float2), groups = (size_t)(G > s.work / 32 * GN_PARAM_COLS ? G : s.work / 32 * GN_PARAM_COLS) * sizeof(float2);
         for (int n = 0; n < N; n += s.unit) {
             p.last = n + s.unit >= N && (dw || db);
             int e = joint ? (codes ? gn_launch<gn_bwd_sums_kernel<T, true, true>>(p, n, sums, st) : gn_launch<gn_bwd_sums_kernel<T, true, false>>(p, n, sums, st))
