@@ -14,12 +14,12 @@
 // Each way is a pass for the sums, which leaves a word per group and tile, and a pass for the results, whose blocks merge their
 // sample's words themselves.  Both read x, so they take turns over units of samples that stay in L2 in between: the first pass asks L2
 // to keep what it reads, the second to let go of what it reads and writes.  Launches are chained (common.cuh), which hides their gaps.
-// Measured, in a graph: 64 x 106 x 106 x 128 fp32 177 us (reading x and writing y once takes 112 at the measured copy rate; part of the
-// second read comes from memory, and a unit's passes each start and drain), 8 x 211 x 211 x 42 bf16 24.8 (9.1; two waves' latencies), 43 x
-// 43 x 128 fp32 8.0 (two launches); backward of 4 x 71 x 71 x 128 fp32 19.4 (4.7), of 16 x 106 x 106 x 128 fp32 from a
-// checkpoint 70.6 (32), of 8 x 211 x 211 x 44 bf16 from one 46.4 (12).
-// One launch in which a cluster of 8 or 16 blocks shares a sample and meets in the middle is no faster: 178 to 191 us for the first,
-// 36.6, 9.5, and 21 to 27, 110, 67 backward.
+// Measured, in a graph, with what reading x (and dy) and writing the result once takes at the measured copy rate: 64 x 106 x 106 x 128
+// fp32 174 us (112; part of the second read comes from memory, and a unit's passes each start and drain), 8 x 211 x 211 x 42 bf16 24.5
+// (9.1; two waves' latencies), 43 x 43 x 128 fp32 7.7 (0.3; two launches); backward of 4 x 71 x 71 x 128 fp32 15.9 (4.7), of 16 x 106 x
+// 106 x 128 fp32 from a checkpoint 64 (32), of 8 x 211 x 211 x 44 bf16 from one 36.3 (12).
+// One launch in which a cluster of 8 or 16 blocks shares a sample and meets in the middle is no faster: 178 to 191 us, 37 and 9.5 for
+// the first three.
 #include "lowp.cuh"
 
 namespace spgt {
@@ -120,18 +120,30 @@ template <class T> __device__ __forceinline__ uint4 gn_raw(const T* p, uint64_t 
     asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy));
     return v;
 }
-// f(loaded) for each of the thread's vectors of a tile: load(j) U at a time, j in vectors from the tile's first.
-template <int U, class L, class F> __device__ __forceinline__ void gn_vectors(const GnTask& t, const GnThread& me, L&& load, F&& f) {
-    if (!me.active) return;
-    int j = me.mine;
-    for (; j + (U - 1) * me.period < t.left; j += U * me.period) {
-        decltype(load(0)) r[U];
+// f(j, loaded) for batches of U of the thread's vectors of a tile, which are j, j + period, ... in vectors from the tile's first; those past
+// its end are for f to leave out.  load() runs B batches ahead, and loads the thread's last vector in the place of those, so that
+// no branch keeps the loads apart.
+template <int U, int B, class L, class F> __device__ __forceinline__ void gn_vectors(const GnTask& t, const GnThread& me, L&& load, F&& f) {
+    if (!me.active || me.mine >= t.left) return;
+    const int period = me.period, last = t.left - 1 - (t.left - 1 - me.mine) % period;
+    decltype(load(0)) r[B][U];
+    auto fetch = [&](decltype(load(0)) (&to)[U], int j) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) r[u] = load(j + u * me.period);
+        for (int u = 0; u < U; ++u) to[u] = load(min(j + u * period, last));
+    };
 #pragma unroll
-        for (int u = 0; u < U; ++u) f(j + u * me.period, r[u]);
+    for (int b = 0; b < B; ++b)
+        if (me.mine + b * U * period < t.left) fetch(r[b], me.mine + b * U * period);
+    for (int j = me.mine; j < t.left; j += B * U * period) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int jb = j + b * U * period;
+            if (jb < t.left) {
+                f(jb, r[b]);
+                if (jb + B * U * period < t.left) fetch(r[b], jb + B * U * period);
+            }
+        }
     }
-    for (; j < t.left; j += me.period) f(j, load(j));
 }
 template <class F> __device__ __forceinline__ void gn_with_act(int act, F&& f) {
     if (act == SPGT_ACT_SILU) f(std::integral_constant<int, SPGT_ACT_SILU>{});
@@ -143,7 +155,7 @@ template <class F> __device__ __forceinline__ void gn_with_act(int act, F&& f) {
 // ---- forward: sums -----------------------------------------------------------------------------------------------------------------
 // JOINT: a vector lies in one group (cg a multiple of V, no head), so its V values are one set; else a set per channel.
 template <class T, bool JOINT> __global__ void __launch_bounds__(GN_MAX_WORK) gn_stats_kernel(const GnParams p) {
-    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V, U = 4, B = 2;     // vectors to a merge, merges to a batch of loads
+    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V, U = 8;      // vectors to a merge
     extern __shared__ float2 s_set[];                       // [R K S] mean, M2
     __shared__ float one[2 * V];
     __shared__ int one_group[2 * V];
@@ -200,19 +212,13 @@ template <class T, bool JOINT> __global__ void __launch_bounds__(GN_MAX_WORK) gn
         }
         n = total;
     };
+    gn_vectors<U, 1>(t, me, [&](int j) { return gn_raw(x + (int64_t)j * V, keep); }, [&](int j, const uint4 (&raw)[U]) {
+        if (j + (U - 1) * period < t.left) { take(std::integral_constant<int, U>{}, raw); return; }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j + u * period < t.left) take(std::integral_constant<int, 1>{}, raw + u);
+    });
     if (me.active) {
-        int j = mine;
-        for (; j + (U * B - 1) * period < t.left; j += U * B * period) {
-            uint4 raw[U * B];
-#pragma unroll
-            for (int u = 0; u < U * B; ++u) raw[u] = gn_raw(x + (int64_t)(j + u * period) * V, keep);
-#pragma unroll
-            for (int k = 0; k < B; ++k) take(std::integral_constant<int, U>{}, raw + U * k);
-        }
-        for (; j < t.left; j += period) {
-            const uint4 raw = gn_raw(x + (int64_t)j * V, keep);
-            take(std::integral_constant<int, 1>{}, &raw);
-        }
 #pragma unroll
         for (int i = 0; i < S; ++i) s_set[mine * S + i] = make_float2(mean[i], m2[i]);
     }
@@ -330,7 +336,7 @@ template <int V, bool JOINT> struct GnChannels {
 
 // ---- forward: y --------------------------------------------------------------------------------------------------------------------
 template <class T, bool JOINT, bool KEEP> __global__ void __launch_bounds__(GN_MAX_WORK) gn_apply_kernel(const GnParams p) {
-    constexpr int V = Pack<T>::N;
+    constexpr int V = Pack<T>::N, U = 6;
     extern __shared__ float2 s_group[];
     pdl_launch_next();
     const GnShape& s = p.s;
@@ -355,20 +361,26 @@ template <class T, bool JOINT, bool KEEP> __global__ void __launch_bounds__(GN_M
             act_values(ACT, z);
             ((T*)p.out)[t.first + at] = from_f32<T>(z[0]);
         }
-        gn_vectors<4>(t, me, [&](int j) { return gn_raw(x + (int64_t)j * V, drop); }, [&](int j, const uint4& raw) {
-            float2 v[V / 2];
-            unpack_pairs(raw, v, T{});
-            const int64_t o = t.base + (int64_t)j * V;
-            // (C a multiple of 32: the lanes that share a block of the checkpoint take part together)
-            if constexpr (KEEP) {
-                float x[V];
+        gn_vectors<U, V == 4 ? 1 : 2>(t, me, [&](int j) { return gn_raw(x + (int64_t)j * V, drop); }, [&](int j0, const uint4 (&batch)[U]) {
 #pragma unroll
-                for (int i = 0; i < V / 2; ++i) { x[2 * i] = v[i].x; x[2 * i + 1] = v[i].y; }
-                q8_store(p.out_codes, p.out_steps, o, x, (Q8_BLOCK / V == 8 ? 0xffu : 0xfu) << (threadIdx.x & 31 & ~(Q8_BLOCK / V - 1)));
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * me.period;
+                if (j >= t.left) break;
+                const uint4 raw = batch[u];
+                float2 v[V / 2];
+                unpack_pairs(raw, v, T{});
+                const int64_t o = t.base + (int64_t)j * V;
+                // (C a multiple of 32: the lanes that share a block of the checkpoint take part together)
+                if constexpr (KEEP) {
+                    float x[V];
+#pragma unroll
+                    for (int i = 0; i < V / 2; ++i) { x[2 * i] = v[i].x; x[2 * i + 1] = v[i].y; }
+                    q8_store(p.out_codes, p.out_steps, o, x, (Q8_BLOCK / V == 8 ? 0xffu : 0xfu) << (threadIdx.x & 31 & ~(Q8_BLOCK / V - 1)));
+                }
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) v[i] = act_value2<ACT>(fma2(add2(v[i], ch.minus_mean(i)), ch.a[i], ch.b[i]));
+                __stcs(reinterpret_cast<uint4*>((T*)p.out + o), pack_pairs(v, T{}));
             }
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) v[i] = act_value2<ACT>(fma2(add2(v[i], ch.minus_mean(i)), ch.a[i], ch.b[i]));
-            __stcs(reinterpret_cast<uint4*>((T*)p.out + o), pack_pairs(v, T{}));
         });
     });
 }
@@ -378,6 +390,10 @@ template <class T, bool CODES> __device__ __forceinline__ float gn_load_single(c
     if constexpr (CODES) return (float)p.codes[at] * q8_step(p.steps[at >> 5]);
     else return to_f32(((const T*)p.x)[at]);
 }
+// Vectors in a batch and batches ahead.  Measured with batches of 2, one at a time, and the rest singly / these: 4 x 71 x 71 x 128 fp32 19.4 /
+// 16.2 us, 16 x 106 x 106 x 128 fp32 from a checkpoint 70.6 / 64, 8 x 211 x 211 x 44 bf16 from one 46.4 / 36.2.
+template <int V> constexpr int GN_BWD_BATCH = V == 4 ? 2 : 6;
+template <int V> constexpr int GN_BWD_AHEAD = V == 4 ? 3 : 1;
 // A vector of dy with its x, as loaded.
 template <int V, bool CODES> struct GnPair { uint4 d; uint4 x; };
 template <int V> struct GnPair<V, true> { uint4 d; uint32_t q[V / 4]; uint32_t e; };
@@ -420,7 +436,7 @@ template <class T, bool CODES, bool JOINT, int V> __device__ __forceinline__ voi
 
 // sums of dz and dz xh of each channel over a tile's pixels, and of w dz and w dz xh of each group
 template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_MAX_WORK) gn_bwd_sums_kernel(const GnParams p) {
-    constexpr int V = Pack<T>::N;
+    constexpr int V = Pack<T>::N, U = GN_BWD_BATCH<V>;
     extern __shared__ float2 s_sum[];                       // [R][K V]
     __shared__ float2 one[2 * V];
     __shared__ int one_channel[2 * V];
@@ -449,14 +465,19 @@ template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_
             one[threadIdx.x] = make_float2(d[0], d[0] * xm);
             one_channel[threadIdx.x] = c;
         }
-        gn_vectors<2>(t, me, [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, keep); }, [&](int, const GnPair<V, CODES>& r) {
-            float2 v[V / 2], d[V / 2];
-            gn_values<T, CODES, JOINT, V>(r, ch, v, d);
+        gn_vectors<U, GN_BWD_AHEAD<V>>(t, me, [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, keep); }, [&](int j0, const GnPair<V, CODES> (&batch)[U]) {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const float2 dz = act_slope2<ACT>(fma2(v[i], ch.a[i], ch.b[i]), d[i]);
-                A[i] = add2(A[i], dz);
-                B[i] = fma2(dz, v[i], B[i]);
+            for (int u = 0; u < U; ++u) {
+                if (j0 + u * me.period >= t.left) break;
+                const GnPair<V, CODES>& r = batch[u];
+                float2 v[V / 2], d[V / 2];
+                gn_values<T, CODES, JOINT, V>(r, ch, v, d);
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) {
+                    const float2 dz = act_slope2<ACT>(fma2(v[i], ch.a[i], ch.b[i]), d[i]);
+                    A[i] = add2(A[i], dz);
+                    B[i] = fma2(dz, v[i], B[i]);
+                }
             }
         });
     });
@@ -534,7 +555,7 @@ __device__ __forceinline__ void gn_params(const GnParams& p, float2* part) {
 }
 
 template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_MAX_WORK) gn_bwd_apply_kernel(const GnParams p) {
-    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V / 2;
+    constexpr int V = Pack<T>::N, S = JOINT ? 1 : V / 2, U = GN_BWD_BATCH<V>;
     extern __shared__ float2 s_group[];
     pdl_launch_next();
     const GnShape& s = p.s;
@@ -570,15 +591,21 @@ template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_
             act_slopes(ACT, z, d);
             ((T*)p.out)[t.first + at] = from_f32<T>(fmaf(xm, -st.y * st.y * k.y, fmaf(a, d[0], -st.y * k.x)));
         }
-        gn_vectors<2>(t, me, [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, drop); }, [&](int j, const GnPair<V, CODES>& r) {
-            float2 v[V / 2], d[V / 2];
-            gn_values<T, CODES, JOINT, V>(r, ch, v, d);
+        gn_vectors<U, GN_BWD_AHEAD<V>>(t, me, [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, drop); }, [&](int j0, const GnPair<V, CODES> (&batch)[U]) {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const float2 dz = act_slope2<ACT>(fma2(v[i], ch.a[i], ch.b[i]), d[i]);
-                d[i] = fma2(v[i], k2[JOINT ? 0 : i], fma2(ch.a[i], dz, k1[JOINT ? 0 : i]));
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * me.period;
+                if (j >= t.left) break;
+                const GnPair<V, CODES>& r = batch[u];
+                float2 v[V / 2], d[V / 2];
+                gn_values<T, CODES, JOINT, V>(r, ch, v, d);
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) {
+                    const float2 dz = act_slope2<ACT>(fma2(v[i], ch.a[i], ch.b[i]), d[i]);
+                    d[i] = fma2(v[i], k2[JOINT ? 0 : i], fma2(ch.a[i], dz, k1[JOINT ? 0 : i]));
+                }
+                __stcs(reinterpret_cast<uint4*>((T*)p.out + t.base + (int64_t)j * V), pack_pairs(d, T{}));
             }
-            __stcs(reinterpret_cast<uint4*>((T*)p.out + t.base + (int64_t)j * V), pack_pairs(d, T{}));
         });
     });
     if (p.last) gn_params(p, s_group);
@@ -606,9 +633,10 @@ static int gn_shape(int N, int64_t P, int C, int G, int dtype, int tensors, bool
     const int samples = N > 0 ? N : 1, units = (int)(unit >= samples ? 1 : ceil_div<int64_t>(samples, unit < 1 ? 1 : unit));
     s.unit = ceil_div(samples, units);                      // (units of nearly the same size)
     // As many tiles as blocks run at a time, so that a pass is one wave and its blocks end together; no tile of less than four rows of
-    // vectors, nor less than twice the words that a block of the second pass merges.  Vectors of eight values take more registers and
-    // more merging per block: two blocks to an SM (8 x 211 x 211 x 42 bf16 with 2 / 3 / 4 / 6: 24.1 / 26.4 / 25.4 / 28.5 us).
-    const int64_t rows = ceil_div<int64_t>(s.L / s.V, (int64_t)s.R * s.K), resident = (int64_t)num_sms() * (s.work > 256 ? 1 : s.V == 8 ? 2 : 4);
+    // vectors, nor less than twice the words that a block of the second pass merges.  Vectors of eight values, and the backward pass's pairs,
+    // take more registers, and blocks more merging: two blocks to an SM (backward of 16 x 106 x 106 x 128 with 2 / 3 / 4: 64 / 77 / 79 us, 8 x
+    // 211 x 211 x 42 bf16 forward 24.6 / 33 / 31; 64 x 106 x 106 x 128 fp32 forward 188 / 180 / 174).
+    const int64_t rows = ceil_div<int64_t>(s.L / s.V, (int64_t)s.R * s.K), resident = (int64_t)num_sms() * (s.work > 256 ? 1 : s.V == 8 || tensors == 2 ? 2 : 4);
     int64_t tiles = resident / s.unit;
     while (tiles > 1 && tiles * tiles * 16 * G > bytes) tiles = tiles * 7 / 8;
     if (tiles > rows / 4) tiles = rows / 4;
