@@ -10,10 +10,10 @@
 // they are added to the block's result in memory.  Error against 64 bits, relative, with normal inputs: 8.8e-8 for 7396 rows and 3.2e-7
 // for 179776, a plain fp32 product's 5e-7 and 1.3e-6.
 // Blocks split the rows; their results are added by a second kernel in order.
-// Bound by shared memory and the copies: a block of 32 rows moves 160 KB through shared memory (copies in, out, parts in, and 12 KB to
-// each MMA, which take the tensor cores 0.4 us), about 0.7 us, against 0.5 us for its 24 KB from memory, and the two overlap in part;
-// then 12 us for the blocks' partial results, their sum and the launches.  179776 rows, dy 128 columns, x 256: fp32 56 us (118 MB in 21
-// us at the measured copy rate), fp16 49, bf16 47; dy 256 columns, x 128: fp32 66; dy 130, x 250: fp32 175; 7396 rows, 128 x 136 bf16: 15.
+// Bound by what the loading warps do: of 179776 rows, dy 128 columns and x 256 in fp32, 53 us, 15 remain without copies, conversion and
+// MMAs (the start, the blocks' partial results and their sum), the copies add 22 (118 MB, at the measured rate 18), the conversion
+// alone 21, and the two overlap little: a block of 32 rows takes 212 instructions of each warp and 1100 cycles of shared memory, besides
+// what the MMAs read.  fp16 47 us, bf16 46; dy 256 columns, x 128: fp32 64; dy 130, x 250: fp32 173; 7396 rows, 128 x 136 bf16: 14.8.
 //   warps 0-15 load and convert, 16-19 write the results, and the first of those issues the MMAs.  Every wait is a bounded mbarrier poll
 // that records a code on expiry.
 #include "lowp.cuh"
@@ -34,7 +34,7 @@ template <class T, int BN> struct W8 {
     static constexpr int STAGE = (P + BN / W8_T) * PART, STAGES = BN == 256 ? (P == 3 ? 3 : 4) : 5 - P;
     // raw values of a block per loading thread: DU times eight columns of dy, in 16-byte pieces, and XU times eight codes
     static constexpr int PIECES = 8 * (int)sizeof(T) / 16, DU = ROWS / 32, XU = ROWS * BN / (8 * W8_LOADERS);
-    static constexpr int RAW = W8_LOADERS * (16 * PIECES * DU + 8 * XU), RAWS = BN == 256 ? 4 : 5 - P;
+    static constexpr int RAW = W8_LOADERS * (16 * PIECES * DU + 8 * XU), RAWS = BN == 256 ? (P == 3 ? 3 : 4) : 5 - P;
     static constexpr int BAR = STAGES * STAGE + RAWS * RAW, SMEM = BAR + W8_BAR, CHAIN = W8_CHAIN / ROWS;
     static constexpr int COLUMNS = (P > 1 ? 2 : 1) * BN;                       // of tensor memory: the upper parts' sums, then the others'
     // where unit c (of eight columns) of row r lies in a part
@@ -126,42 +126,41 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
             const bool n_in = nc < p.N, n2_in = PIECES == 2 && nc + 64 < p.N, k_in = k0 + kc * 8 < p.K;
             uint8_t* raw = smem + STAGES * STAGE + tid * 16;
             uint8_t* raw_codes = smem + STAGES * STAGE + DU * PIECES * (W8_LOADERS * 16) + tid * 8;
-            const int64_t end = (first + mine) * ROWS < p.rows ? (first + mine) * ROWS : p.rows, dy_row = (int64_t)p.N * (int)sizeof(T);
-            int64_t row = first * ROWS;                     // of the block to copy
-            const uint8_t* dy_at = (const uint8_t*)p.dy + (row + r) * dy_row + (int64_t)nc * (int)sizeof(T);
-            int64_t at = (row + kr) * p.K + k0 + kc * 8;    // value of x
-            int slot_in = 0, slot_out = 0;
+            const int64_t end = (first + mine) * ROWS < p.rows ? (first + mine) * ROWS : p.rows, dy_row = (int64_t)p.N * (int)sizeof(T), x_step = (int64_t)KSTEP * p.K;
+            // rows left at the thread's first row of the block to copy (a copy of no bytes touches no address)
+            int dy_left = (int)(end - first * ROWS) - r, x_left = (int)(end - first * ROWS) - kr;
+            const uint8_t* dy_at = (const uint8_t*)p.dy + (first * ROWS + r) * dy_row + (int64_t)nc * (int)sizeof(T);
+            int64_t at = (first * ROWS + kr) * p.K + k0 + kc * 8;        // value of x
             // the steps are loaded with the copies and held until their block's turn
             uint32_t e[RAWS][XU];
-            auto copy = [&](uint32_t (&step)[XU]) {
-                uint8_t* to = raw + slot_in * W::RAW;
+            auto copy = [&](int slot) {
 #pragma unroll
                 for (int u = 0; u < DU; ++u) {
-                    const bool in = row + r + 32 * u < end;
+                    const bool in = 32 * u < dy_left;
+                    uint8_t* to = raw + slot * W::RAW + u * PIECES * (W8_LOADERS * 16);
                     const uint8_t* from = dy_at + 32 * u * dy_row;
-                    cp_async_zfill<16>(to + u * PIECES * (W8_LOADERS * 16), in && n_in ? from : (const uint8_t*)p.dy, in && n_in);
-                    if constexpr (PIECES == 2) cp_async_zfill<16>(to + (2 * u + 1) * (W8_LOADERS * 16), in && n2_in ? from + 256 : (const uint8_t*)p.dy, in && n2_in);
+                    cp_async_zfill<16>(to, from, in && n_in);
+                    if constexpr (PIECES == 2) cp_async_zfill<16>(to + W8_LOADERS * 16, from + 256, in && n2_in);
                 }
 #pragma unroll
                 for (int u = 0; u < XU; ++u) {
-                    const bool there = k_in && row + kr + KSTEP * u < end;
-                    const int64_t from = there ? at + KSTEP * u * (int64_t)p.K : 0;
-                    cp_async_zfill<8>(raw_codes + slot_in * W::RAW + u * (W8_LOADERS * 8), p.codes + from, there);
-                    step[u] = there ? __ldg(p.steps + (from >> 5)) : 1u;
+                    const bool there = k_in && KSTEP * u < x_left;
+                    const int64_t from = at + u * x_step;
+                    cp_async_zfill<8>(raw_codes + slot * W::RAW + u * (W8_LOADERS * 8), p.codes + from, there);
+                    e[slot][u] = there ? __ldg(p.steps + (from >> 5)) : 1u;
                 }
                 cp_async_commit();
-                row += ROWS; dy_at += ROWS * dy_row; at += ROWS * (int64_t)p.K;
-                slot_in = slot_in == RAWS - 1 ? 0 : slot_in + 1;
+                dy_left -= ROWS; x_left -= ROWS; dy_at += ROWS * dy_row; at += XU * x_step;
             };
             if (mine > 0) {
 #pragma unroll
-                for (int k = 0; k < RAWS; ++k) copy(e[k]);
+                for (int k = 0; k < RAWS; ++k) copy(k);
             }
-            auto step = [&](uint32_t (&size)[XU]) {
+            auto step = [&](int slot) {
                 cp_async_wait<RAWS - 1>();
                 if (!__all_sync(0xffffffffu, mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status))) return false;
                 uint8_t* stage = smem + s * STAGE;
-                const uint8_t* from = raw + slot_out * W::RAW;
+                const uint8_t* from = raw + slot * W::RAW;
 #pragma unroll
                 for (int u = 0; u < DU; ++u) {
                     float2 b[4];
@@ -193,9 +192,9 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
                 }
 #pragma unroll
                 for (int u = 0; u < XU; ++u) {
-                    const uint2 q = *reinterpret_cast<const uint2*>(raw_codes + slot_out * W::RAW + u * (W8_LOADERS * 8));
+                    const uint2 q = *reinterpret_cast<const uint2*>(raw_codes + slot * W::RAW + u * (W8_LOADERS * 8));
                     const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
-                    const float2 scale = pair(q8_step(size[u]));
+                    const float2 scale = pair(q8_step(e[slot][u]));
                     float2 y[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -205,8 +204,7 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
                     }
                     *reinterpret_cast<uint4*>(stage + P * PART + W::at(kr + KSTEP * u, kc)) = pack_pairs(y, __nv_bfloat16{});
                 }
-                slot_out = slot_out == RAWS - 1 ? 0 : slot_out + 1;
-                copy(size);
+                copy(slot);
                 stored();
                 return true;
             };
@@ -214,7 +212,7 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
             for (int k = 0; k < mine && alive; k += RAWS) {
 #pragma unroll
                 for (int j = 0; j < RAWS; ++j)
-                    if (alive && k + j < mine) alive = step(e[j]);
+                    if (alive && k + j < mine) alive = step(j);
             }
             cp_async_wait_all();
         } else {
