@@ -1131,7 +1131,7 @@ extern "C" int spgt_tc_status(void) {
     if (int e = spgt::encoder_out_status(false)) return e;      // 60..76: its second half
     if (int e = spgt::conv_status(false)) return e;             // 80..86: the convolution kernel
     if (int e = spgt::tn_status(false)) return e;               // 90..96: the weight-gradient kernel
-    if (int e = spgt::w8_status(false)) return e;               // 130..134: weight gradients from a checkpoint
+    if (int e = spgt::w8_status(false)) return e;               // 130..136: weight gradients from a checkpoint
     return spgt::ffn_tc_status();               // 21..34: a wait of the fused feed-forward kernel gave up
 }
 

@@ -10,12 +10,12 @@
 // they are added to the block's result in memory.  Error against 64 bits, relative, with normal inputs: 8.8e-8 for 7396 rows and 3.2e-7
 // for 179776, a plain fp32 product's 5e-7 and 1.3e-6.
 // Blocks split the rows; their results are added by a second kernel in order.
-// Bound by what the loading warps do: of 179776 rows, dy 128 columns and x 256 in fp32, 53 us, 15 remain without copies, conversion and
-// MMAs (the start, the blocks' partial results and their sum), the copies add 22 (118 MB, at the measured rate 18), the conversion
-// alone 21, and the two overlap little: a block of 32 rows takes 212 instructions of each warp and 1100 cycles of shared memory, besides
-// what the MMAs read.  fp16 47 us, bf16 46; dy 256 columns, x 128: fp32 64; dy 130, x 250: fp32 173; 7396 rows, 128 x 136 bf16: 14.8.
-//   warps 0-15 load and convert, 16-19 write the results, and the first of those issues the MMAs.  Every wait is a bounded mbarrier poll
-// that records a code on expiry.
+// Bound by what the loading warps do: of 179776 rows, dy 128 columns and x 256 in fp32, 42 us, about 10 are the start, the blocks' partial
+// results and their sum; the copies alone take 22 (118 MB, at the measured rate 18), conversion alone about as long (a block of 32 rows,
+// of which a multiprocessor has 38, is split, stored and multiplied in some 0.8 us), and the two overlap in part.  fp16 36 us, bf16 33; dy 256
+// columns, x 128: fp32 59; dy 130, x 250: fp32 165; 7396 rows, 128 x 136 bf16: 11.
+//   Warps 0-15 load and convert, 16-19 write the results, the first of those issues the MMAs, and 20 copies where blocks are runs of
+// memory (W8_WHOLE).  Every wait is a bounded mbarrier poll that records a code on expiry.
 #include "lowp.cuh"
 
 namespace spgt {
@@ -27,14 +27,22 @@ constexpr int W8_T = 128, W8_THREADS = 640, W8_LOADERS = 512, W8_BAR = 256, W8_C
 template <class T> struct W8Parts { static constexpr int N = 3; };
 template <> struct W8Parts<__half> { static constexpr int N = 2; };
 template <> struct W8Parts<__nv_bfloat16> { static constexpr int N = 1; };
+// How the blocks of rows are read.  W8_ANY: any widths.  W8_VEC: N and K are multiples of eight, so eight columns of a row are in or out
+// together and start on a boundary of their size.  W8_WHOLE: besides, one tile holds all columns, so that a block is three runs of memory,
+// which bulk copies bring, and K is a multiple of 16 (179776 rows, 128 x 256 columns: fp32 47 us against 53, bf16 38 against 46; dy 256
+// columns, x 128 with a copy for each row of dy 113 against 64).
+constexpr int W8_ANY = 0, W8_VEC = 1, W8_WHOLE = 2;
 // BN: columns of x in a tile, 128 or 256, and with it rows of a block.
-template <class T, int BN> struct W8 {
+template <class T, int BN, int MODE> struct W8 {
     static constexpr int P = W8Parts<T>::N, ROWS = BN == 256 ? 32 : 64;
     static constexpr int HALF = ROWS * 128, PART = 2 * HALF;                   // 64 columns of a block's rows: lines of 128 bytes; 128 columns
     static constexpr int STAGE = (P + BN / W8_T) * PART, STAGES = BN == 256 ? (P == 3 ? 3 : 4) : 5 - P;
     // raw values of a block per loading thread: DU times eight columns of dy, in 16-byte pieces, and XU times eight codes
     static constexpr int PIECES = 8 * (int)sizeof(T) / 16, DU = ROWS / 32, XU = ROWS * BN / (8 * W8_LOADERS);
-    static constexpr int RAW = W8_LOADERS * (16 * PIECES * DU + 8 * XU), RAWS = BN == 256 ? (P == 3 ? 3 : 4) : 5 - P;
+    static constexpr int RAW_CODES = ROWS * W8_T * (int)sizeof(T), RAW_STEPS = RAW_CODES + ROWS * BN;      // W8_WHOLE: dy, codes and steps as they are
+    static constexpr int RAW = MODE == W8_WHOLE ? RAW_STEPS + ROWS * BN / Q8_BLOCK : W8_LOADERS * (16 * PIECES * DU + 8 * XU);
+    static constexpr int RAWS = MODE != W8_WHOLE ? (BN == 256 ? (P == 3 ? 3 : 4) : 5 - P) : BN == 256 ? (P == 3 ? 4 : 6) : P == 3 ? 2 : P == 2 ? 3 : 4;
+    static constexpr int THREADS = W8_THREADS + (MODE == W8_WHOLE ? 32 : 0);
     static constexpr int BAR = STAGES * STAGE + RAWS * RAW, SMEM = BAR + W8_BAR, CHAIN = W8_CHAIN / ROWS;
     static constexpr int COLUMNS = (P > 1 ? 2 : 1) * BN;                       // of tensor memory: the upper parts' sums, then the others'
     // where unit c (of eight columns) of row r lies in a part
@@ -43,12 +51,12 @@ template <class T, int BN> struct W8 {
     static __device__ __forceinline__ uint64_t desc(uint32_t smem) {
         return (uint64_t)((smem >> 4) & 0x3fffu) | ((uint64_t)(HALF >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
     }
-    static_assert(SMEM <= 227 * 1024 && 8 * (2 * STAGES + 2) <= 96, "shared memory budget");
+    static_assert(SMEM <= 227 * 1024 && 8 * (2 * STAGES + 2) <= 96 && 128 + 8 * 2 * RAWS <= W8_BAR && RAW % 16 == 0, "shared memory budget");
 };
 
 struct W8Params {
     const void* dy; const int8_t* codes; const uint8_t* steps;
-    float *partial, *colpart;           // [split][tile][128][BN], [split][row of tiles][128]
+    float *partial, *colpart;           // [split][tile][BN / 4][128][4], [split][row of tiles][128]
     float *dw, *db;
     int N, K, kt, splits;               // kt: tiles along K
     int64_t rows;
@@ -72,9 +80,13 @@ template <int BN> __device__ __forceinline__ void w8_mma(uint32_t d, uint64_t a,
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// VEC: N and K are multiples of eight, so eight columns of a row are in or out together and start on a boundary of their size.
-template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREADS, 1) weight_gradient8_kernel(const W8Params p) {
-    using W = W8<T, BN>;
+// a run of memory to shared memory, counted by an mbarrier; 16-byte boundaries and sizes
+__device__ __forceinline__ void w8_bulk(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <class T, int MODE, int BN> __global__ void __launch_bounds__(W8<T, BN, MODE>::THREADS, 1) weight_gradient8_kernel(const W8Params p) {
+    using W = W8<T, BN, MODE>;
     constexpr int P = W::P, STAGES = W::STAGES, STAGE = W::STAGE, PIECES = W::PIECES, DU = W::DU, XU = W::XU, RAWS = W::RAWS, ROWS = W::ROWS, HALF = W::HALF, PART = W::PART;
     extern __shared__ __align__(1024) uint8_t smem[];
     pdl_launch_next();                                      // (the second kernel waits for the end of this one)
@@ -86,6 +98,8 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
     auto st_full = [&](uint32_t s) { return bars + 8u * s; };
     auto st_empty = [&](uint32_t s) { return bars + 8u * (STAGES + s); };
     const uint32_t acc_full = bars + 8u * (2 * STAGES), acc_empty = acc_full + 8u;
+    auto raw_full = [&](uint32_t s) { return bars + 128u + 8u * s; };
+    auto raw_empty = [&](uint32_t s) { return bars + 128u + 8u * (RAWS + s); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + W::BAR + 96);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + W::BAR + 104);
     const int tid = threadIdx.x, warp = (int)tc_uniform(tid >> 5), lane = tid & 31;
@@ -95,6 +109,8 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(st_full(s), W8_LOADERS / 32); mbar_init(st_empty(s), 1); }
         mbar_init(acc_full, 1); mbar_init(acc_empty, 128);
+        if constexpr (MODE == W8_WHOLE)
+            for (int s = 0; s < RAWS; ++s) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), W8_LOADERS / 32); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -117,104 +133,142 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
             if (lane == 0) mbar_arrive(st_full(s));
             if (++s == STAGES) { s = 0; ph ^= 1u; }
         };
-        if constexpr (VEC) {
-            // dy: unit c of rows r, r + 32; fp32: columns 4 c .. + 3 and 64 + 4 c .. + 3, so that the lanes' 16-byte copies are next to each
-            // other.  x: unit kc of rows kr, kr + KSTEP.  Each thread copies what it will convert, RAWS blocks ahead, and only waits for itself.
+        if constexpr (MODE != W8_ANY) {
+            // dy: unit c of rows r, r + 32; fp32: columns 4 c .. + 3 and 64 + 4 c .. + 3, so that the lanes' 16-byte accesses are next to each
+            // other.  x: unit kc of rows kr, kr + KSTEP.
             constexpr int KSTEP = ROWS / XU;
             const int c = tid & 15, r = tid >> 4, kc = BN == 256 ? tid & 31 : c, kr = BN == 256 ? tid >> 5 : r;
             const int nc = n0 + c * (16 / (int)sizeof(T));
             const bool n_in = nc < p.N, n2_in = PIECES == 2 && nc + 64 < p.N, k_in = k0 + kc * 8 < p.K;
-            uint8_t* raw = smem + STAGES * STAGE + tid * 16;
-            uint8_t* raw_codes = smem + STAGES * STAGE + DU * PIECES * (W8_LOADERS * 16) + tid * 8;
-            const int64_t end = (first + mine) * ROWS < p.rows ? (first + mine) * ROWS : p.rows, dy_row = (int64_t)p.N * (int)sizeof(T), x_step = (int64_t)KSTEP * p.K;
-            // rows left at the thread's first row of the block to copy (a copy of no bytes touches no address)
+            const int64_t end = (first + mine) * ROWS < p.rows ? (first + mine) * ROWS : p.rows;
+            // rows left at the thread's first row of a block
             int dy_left = (int)(end - first * ROWS) - r, x_left = (int)(end - first * ROWS) - kr;
-            const uint8_t* dy_at = (const uint8_t*)p.dy + (first * ROWS + r) * dy_row + (int64_t)nc * (int)sizeof(T);
-            int64_t at = (first * ROWS + kr) * p.K + k0 + kc * 8;        // value of x
-            // the steps are loaded with the copies and held until their block's turn
-            uint32_t e[RAWS][XU];
-            auto copy = [&](int slot) {
-#pragma unroll
-                for (int u = 0; u < DU; ++u) {
-                    const bool in = 32 * u < dy_left;
-                    uint8_t* to = raw + slot * W::RAW + u * PIECES * (W8_LOADERS * 16);
-                    const uint8_t* from = dy_at + 32 * u * dy_row;
-                    cp_async_zfill<16>(to, from, in && n_in);
-                    if constexpr (PIECES == 2) cp_async_zfill<16>(to + W8_LOADERS * 16, from + 256, in && n2_in);
+            auto put_dy = [&](uint8_t* stage, int u, const uint4 (&piece)[PIECES]) {
+                float2 b[4];
+                if constexpr (PIECES == 2) {
+                    float2 h[2];
+                    unpack_pairs(piece[0], h, 0.0f);
+                    b[0] = h[0]; b[1] = h[1];
+                    unpack_pairs(piece[PIECES - 1], h, 0.0f);
+                    b[2] = h[0]; b[3] = h[1];
+                } else {
+                    unpack_pairs(piece[0], b, T{});
                 }
 #pragma unroll
-                for (int u = 0; u < XU; ++u) {
-                    const bool there = k_in && KSTEP * u < x_left;
-                    const int64_t from = at + u * x_step;
-                    cp_async_zfill<8>(raw_codes + slot * W::RAW + u * (W8_LOADERS * 8), p.codes + from, there);
-                    e[slot][u] = there ? __ldg(p.steps + (from >> 5)) : 1u;
-                }
-                cp_async_commit();
-                dy_left -= ROWS; x_left -= ROWS; dy_at += ROWS * dy_row; at += XU * x_step;
-            };
-            if (mine > 0) {
+                for (int j = 0; j < 4; ++j) sums[j] = add2(sums[j], b[j]);
+                const uint32_t to = PIECES == 2 ? W::at(r + 32 * u, c >> 1) + (c & 1) * 8 : W::at(r + 32 * u, c);
 #pragma unroll
-                for (int k = 0; k < RAWS; ++k) copy(k);
-            }
-            auto step = [&](int slot) {
-                cp_async_wait<RAWS - 1>();
-                if (!__all_sync(0xffffffffu, mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status))) return false;
-                uint8_t* stage = smem + s * STAGE;
-                const uint8_t* from = raw + slot * W::RAW;
-#pragma unroll
-                for (int u = 0; u < DU; ++u) {
-                    float2 b[4];
+                for (int q = 0; q < P; ++q) {
                     if constexpr (PIECES == 2) {
-                        float2 h[2];
-                        unpack_pairs(*reinterpret_cast<const uint4*>(from + 2 * u * (W8_LOADERS * 16)), h, 0.0f);
-                        b[0] = h[0]; b[1] = h[1];
-                        unpack_pairs(*reinterpret_cast<const uint4*>(from + (2 * u + 1) * (W8_LOADERS * 16)), h, 0.0f);
-                        b[2] = h[0]; b[3] = h[1];
+                        *reinterpret_cast<uint2*>(stage + q * PART + to) = make_uint2(w8_upper(b[0]), w8_upper(b[1]));
+                        *reinterpret_cast<uint2*>(stage + q * PART + HALF + to) = make_uint2(w8_upper(b[2]), w8_upper(b[3]));
                     } else {
-                        unpack_pairs(*reinterpret_cast<const uint4*>(from + u * (W8_LOADERS * 16)), b, T{});
+                        *reinterpret_cast<uint4*>(stage + q * PART + to) = w8_upper(b);
                     }
+                    if (q + 1 < P) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sums[j] = add2(sums[j], b[j]);
-                    const uint32_t to = PIECES == 2 ? W::at(r + 32 * u, c >> 1) + (c & 1) * 8 : W::at(r + 32 * u, c);
-#pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        if constexpr (PIECES == 2) {
-                            *reinterpret_cast<uint2*>(stage + q * PART + to) = make_uint2(w8_upper(b[0]), w8_upper(b[1]));
-                            *reinterpret_cast<uint2*>(stage + q * PART + HALF + to) = make_uint2(w8_upper(b[2]), w8_upper(b[3]));
-                        } else {
-                            *reinterpret_cast<uint4*>(stage + q * PART + to) = w8_upper(b);
-                        }
-                        if (q + 1 < P) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) b[j] = w8_rest(b[j]);
-                        }
+                        for (int j = 0; j < 4; ++j) b[j] = w8_rest(b[j]);
                     }
                 }
-#pragma unroll
-                for (int u = 0; u < XU; ++u) {
-                    const uint2 q = *reinterpret_cast<const uint2*>(raw_codes + slot * W::RAW + u * (W8_LOADERS * 8));
-                    const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
-                    const float2 scale = pair(q8_step(e[slot][u]));
-                    float2 y[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t v = w[j >> 1];
-                        const float2 code = make_float2(__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + 2 * (j & 1))), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7541 + 2 * (j & 1))));
-                        y[j] = mul2(add2(code, pair(-8388736.0f)), scale);
-                    }
-                    *reinterpret_cast<uint4*>(stage + P * PART + W::at(kr + KSTEP * u, kc)) = pack_pairs(y, __nv_bfloat16{});
-                }
-                copy(slot);
-                stored();
-                return true;
             };
-            bool alive = true;
-            for (int k = 0; k < mine && alive; k += RAWS) {
+            auto put_x = [&](uint8_t* stage, int u, uint2 q, uint32_t e) {
+                const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
+                const float2 scale = pair(q8_step(e));
+                float2 y[4];
 #pragma unroll
-                for (int j = 0; j < RAWS; ++j)
-                    if (alive && k + j < mine) alive = step(j);
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t v = w[j >> 1];
+                    const float2 code = make_float2(__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + 2 * (j & 1))), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7541 + 2 * (j & 1))));
+                    y[j] = mul2(add2(code, pair(-8388736.0f)), scale);
+                }
+                *reinterpret_cast<uint4*>(stage + P * PART + W::at(kr + KSTEP * u, kc)) = pack_pairs(y, __nv_bfloat16{});
+            };
+            if constexpr (MODE == W8_WHOLE) {
+                // what warp 20 has copied
+                const uint32_t dy_row = (uint32_t)p.N * (uint32_t)sizeof(T), dy_at = r * dy_row + nc * (uint32_t)sizeof(T), x_at = (uint32_t)(kr * p.K + kc * 8), x_step = (uint32_t)(KSTEP * p.K);
+                uint32_t slot = 0, slot_ph = 0;
+                for (int k = 0; k < mine; ++k) {
+                    const bool there = mbar_wait(raw_full(slot), slot_ph, abort_flag, 135, &g_w8_status) && mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status);
+                    if (!__all_sync(0xffffffffu, there)) break;
+                    uint8_t* stage = smem + s * STAGE;
+                    const uint8_t* from = smem + STAGES * STAGE + slot * W::RAW;
+#pragma unroll
+                    for (int u = 0; u < DU; ++u) {
+                        uint4 piece[PIECES];
+                        const uint8_t* at = from + dy_at + 32u * u * dy_row;
+                        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+                        piece[0] = n_in && 32 * u < dy_left ? *reinterpret_cast<const uint4*>(at) : zero;
+                        if constexpr (PIECES == 2) piece[1] = n2_in && 32 * u < dy_left ? *reinterpret_cast<const uint4*>(at + 256) : zero;
+                        put_dy(stage, u, piece);
+                    }
+#pragma unroll
+                    for (int u = 0; u < XU; ++u) {
+                        const bool in = k_in && KSTEP * u < x_left;
+                        const uint32_t at = x_at + u * x_step;
+                        put_x(stage, u, in ? *reinterpret_cast<const uint2*>(from + W::RAW_CODES + at) : make_uint2(0u, 0u), in ? from[W::RAW_STEPS + at / Q8_BLOCK] : 1u);
+                    }
+                    dy_left -= ROWS; x_left -= ROWS;
+                    stored();
+                    if (lane == 0) mbar_arrive(raw_empty(slot));
+                    if (++slot == RAWS) { slot = 0; slot_ph ^= 1u; }
+                }
+            } else {
+                // Each thread copies what it will convert, RAWS blocks ahead, and only waits for itself.  (A copy of no bytes touches no address.)
+                uint8_t* raw = smem + STAGES * STAGE + tid * 16;
+                uint8_t* raw_codes = smem + STAGES * STAGE + DU * PIECES * (W8_LOADERS * 16) + tid * 8;
+                const int64_t dy_row = (int64_t)p.N * (int)sizeof(T), x_step = (int64_t)KSTEP * p.K;
+                const uint8_t* dy_at = (const uint8_t*)p.dy + (first * ROWS + r) * dy_row + (int64_t)nc * (int)sizeof(T);
+                int64_t at = (first * ROWS + kr) * p.K + k0 + kc * 8;        // value of x
+                uint32_t e[RAWS][XU];                       // the steps are loaded with the copies and held until their block's turn
+                auto copy = [&](int slot) {
+#pragma unroll
+                    for (int u = 0; u < DU; ++u) {
+                        const bool in = 32 * u < dy_left;
+                        uint8_t* to = raw + slot * W::RAW + u * PIECES * (W8_LOADERS * 16);
+                        const uint8_t* from = dy_at + 32 * u * dy_row;
+                        cp_async_zfill<16>(to, from, in && n_in);
+                        if constexpr (PIECES == 2) cp_async_zfill<16>(to + W8_LOADERS * 16, from + 256, in && n2_in);
+                    }
+#pragma unroll
+                    for (int u = 0; u < XU; ++u) {
+                        const bool there = k_in && KSTEP * u < x_left;
+                        const int64_t from = at + u * x_step;
+                        cp_async_zfill<8>(raw_codes + slot * W::RAW + u * (W8_LOADERS * 8), p.codes + from, there);
+                        e[slot][u] = there ? __ldg(p.steps + (from >> 5)) : 1u;
+                    }
+                    cp_async_commit();
+                    dy_left -= ROWS; x_left -= ROWS; dy_at += ROWS * dy_row; at += XU * x_step;
+                };
+                if (mine > 0) {
+#pragma unroll
+                    for (int k = 0; k < RAWS; ++k) copy(k);
+                }
+                auto step = [&](int slot) {
+                    cp_async_wait<RAWS - 1>();
+                    if (!__all_sync(0xffffffffu, mbar_wait(st_empty(s), ph, abort_flag, 131, &g_w8_status))) return false;
+                    uint8_t* stage = smem + s * STAGE;
+#pragma unroll
+                    for (int u = 0; u < DU; ++u) {
+                        uint4 piece[PIECES];
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) piece[i] = *reinterpret_cast<const uint4*>(raw + slot * W::RAW + (u * PIECES + i) * (W8_LOADERS * 16));
+                        put_dy(stage, u, piece);
+                    }
+#pragma unroll
+                    for (int u = 0; u < XU; ++u)
+                        put_x(stage, u, *reinterpret_cast<const uint2*>(raw_codes + slot * W::RAW + u * (W8_LOADERS * 8)), e[slot][u]);
+                    copy(slot);
+                    stored();
+                    return true;
+                };
+                bool alive = true;
+                for (int k = 0; k < mine && alive; k += RAWS) {
+#pragma unroll
+                    for (int j = 0; j < RAWS; ++j)
+                        if (alive && k + j < mine) alive = step(j);
+                }
+                cp_async_wait_all();
             }
-            cp_async_wait_all();
         } else {
             // Any widths: columns 2 lane, 2 lane + 1 (+ 64, ...) of rows warp, warp + 16, ...  Every load has an address inside its array and is
             // zeroed afterwards where it lies outside the tile, so that no branch keeps the loads apart.
@@ -267,11 +321,37 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
                 if (r0 + 32 >= ROWS) stored();
             }
         }
+    } else if (MODE == W8_WHOLE && warp == 20) {
+        // ------------------------------------------ copy (W8_WHOLE) ------------------------------------------
+        const uint32_t dy_row = (uint32_t)p.N * (uint32_t)sizeof(T);
+        uint32_t slot = 0, ph = 1;
+        int k = 0;
+        for (; k < mine; ++k) {
+            if (!__all_sync(0xffffffffu, mbar_wait(raw_empty(slot), ph, abort_flag, 136, &g_w8_status))) break;
+            const int64_t row = (first + k) * ROWS;
+            const uint32_t n = (uint32_t)(p.rows - row < ROWS ? p.rows - row : ROWS), codes = n * (uint32_t)p.K;
+            const uint32_t steps = (codes + Q8_BLOCK - 1) / Q8_BLOCK, most = steps & ~15u;       // the last block's may end off a boundary
+            const uint32_t to = (uint32_t)(STAGES * STAGE) + slot * (uint32_t)W::RAW;
+            const uint8_t* from = p.steps + row * p.K / Q8_BLOCK;
+            if (most + lane < steps) smem[to + W::RAW_STEPS + most + lane] = from[most + lane];
+            __syncwarp();
+            if (lane == 0) {
+                const uint32_t bar = raw_full(slot);
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * dy_row + codes + most) : "memory");
+                w8_bulk(base + to, (const T*)p.dy + row * p.N, n * dy_row, bar);
+                w8_bulk(base + to + W::RAW_CODES, p.codes + row * p.K, codes, bar);
+                if (most > 0) w8_bulk(base + to + W::RAW_STEPS, from, most, bar);
+            }
+            if (++slot == RAWS) { slot = 0; ph ^= 1u; }
+        }
+        // nothing is in flight when the block ends, come what may
+        volatile int none = 0;
+        for (int i = k > RAWS ? k - RAWS : 0; i < k; ++i) mbar_wait(raw_full(i % RAWS), (uint32_t)(i / RAWS) & 1u, &none, 136);
     } else {
         // ------------------------------------------ MMAs and results ------------------------------------------
         const int chains = mine > 0 ? (mine + W::CHAIN - 1) / W::CHAIN : 0;
         uint32_t s = 0, ph = 0;
-        float* out = p.partial + (((int64_t)blockIdx.x * gridDim.y + tile) * W8_T + (warp - 16) * 32 + lane) * BN;
+        float* out = p.partial + (((int64_t)blockIdx.x * gridDim.y + tile) * (BN / 4) * W8_T + (warp - 16) * 32 + lane) * 4;
         const uint32_t row = tmem_base + ((uint32_t)((warp - 16) * 32) << 16);
         // one thread: the MMAs of a chain's blocks of rows
         auto issue = [&](int chain) {
@@ -307,19 +387,19 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
                 float v[16];
                 if constexpr (P > 1) tc_ld16_sum(row + j, BN, v);
                 else tc_ld16(row + j, v);
-                float4* to = reinterpret_cast<float4*>(out + j);
+                float4* to = reinterpret_cast<float4*>(out + j * W8_T);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float4 u = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    if (k > 0) { const float4 w = to[i]; u.x += w.x; u.y += w.y; u.z += w.z; u.w += w.w; }
-                    to[i] = u;
+                    if (k > 0) { const float4 w = to[i * W8_T]; u.x += w.x; u.y += w.y; u.z += w.z; u.w += w.w; }
+                    to[i * W8_T] = u;
                 }
             }
             tc_fence_before();
             mbar_arrive(acc_empty);
         }
         if (chains == 0)                                    // no rows
-            for (int j = 0; j < BN; j += 4) *reinterpret_cast<float4*>(out + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int j = 0; j < BN; j += 4) *reinterpret_cast<float4*>(out + j * W8_T) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     tc_fence_before();
     __syncthreads();
@@ -330,9 +410,9 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
     // column sums of dy, of several threads each; the stages are free
     if (k0 == 0 && p.db) {
         float* part = reinterpret_cast<float*>(smem);
-        constexpr int SHARES = VEC ? 32 : 16;
+        constexpr int SHARES = MODE != W8_ANY ? 32 : 16;
         if (warp < 16) {
-            if constexpr (VEC) {
+            if constexpr (MODE != W8_ANY) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     part[(tid >> 4) * W8_T + (PIECES == 2 ? (tid & 15) * 4 + (j >> 2) * 64 + (j & 3) : (tid & 15) * 8 + j)] = j & 1 ? sums[j / 2].y : sums[j / 2].x;
@@ -351,23 +431,25 @@ template <class T, bool VEC, int BN> __global__ void __launch_bounds__(W8_THREAD
     }
 }
 
-// dw and db from the splits' results.  Eight threads share a result (four columns of a row, or a column sum): thread g adds results g,
-// g + 8, ..., and the eight sums are added in order.
-template <int BN> __global__ void __launch_bounds__(256) weight_gradient8_reduce_kernel(const W8Params p, int tiles) {
-    __shared__ float4 part[8][32];
+// dw and db from the splits' results.  W8_SHARES threads share a result (four columns of a row, or a column sum): thread g adds results g,
+// g + W8_SHARES, ..., and their sums are added in order.  (16 threads with ten loads at a time: one round for 148 splits; 8 threads with
+// eight took 1.5 us more.)
+constexpr int W8_SHARES = 16;
+template <int BN> __global__ void __launch_bounds__(32 * W8_SHARES) weight_gradient8_reduce_kernel(const W8Params p, int tiles) {
+    __shared__ float4 part[W8_SHARES][32];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c_blocks = tiles * (W8_T * BN / 4 / 32);
     pdl_launch_next();
     pdl_wait();
     if ((int)blockIdx.x < c_blocks) {
-        const int i = blockIdx.x * 32 + lane;               // of the padded [tiles][128][BN / 4]
-        const int c4 = i % (BN / 4), r = i / (BN / 4) % W8_T, tile = i / (W8_T * BN / 4);
+        const int i = blockIdx.x * 32 + lane;               // of the padded [tiles][BN / 4][128]
+        const int r = i % W8_T, c4 = i / W8_T % (BN / 4), tile = i / (W8_T * BN / 4);
         const int row = tile / p.kt * W8_T + r, col = tile % p.kt * BN + c4 * 4;
         const bool in = row < p.N && col < p.K;
         const float4* src = reinterpret_cast<const float4*>(p.partial) + i;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         if (in)
-#pragma unroll 8
-            for (int k = g; k < p.splits; k += 8) {
+#pragma unroll 10
+            for (int k = g; k < p.splits; k += W8_SHARES) {
                 const float4 v = __ldcg(src + (int64_t)k * tiles * (W8_T * BN / 4));
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
@@ -375,7 +457,7 @@ template <int BN> __global__ void __launch_bounds__(256) weight_gradient8_reduce
         __syncthreads();
         if (g || !in) return;
 #pragma unroll
-        for (int k = 1; k < 8; ++k) { const float4 v = part[k][lane]; s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
+        for (int k = 1; k < W8_SHARES; ++k) { const float4 v = part[k][lane]; s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
         const float o[4] = {s.x, s.y, s.z, s.w};
         float* dst = p.dw + (int64_t)row * p.K + col;
 #pragma unroll
@@ -384,13 +466,13 @@ template <int BN> __global__ void __launch_bounds__(256) weight_gradient8_reduce
     } else {
         const int c = (blockIdx.x - c_blocks) * 32 + lane;  // (whole tiles of columns)
         float s = 0.0f;
-#pragma unroll 8
-        for (int k = g; k < p.splits; k += 8) s += __ldcg(p.colpart + (int64_t)k * (tiles / p.kt) * W8_T + c);
+#pragma unroll 10
+        for (int k = g; k < p.splits; k += W8_SHARES) s += __ldcg(p.colpart + (int64_t)k * (tiles / p.kt) * W8_T + c);
         part[g][lane].x = s;
         __syncthreads();
         if (g || c >= p.N) return;
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += part[k][lane].x;
+        for (int k = 1; k < W8_SHARES; ++k) s += part[k][lane].x;
         p.db[c] = s;
     }
 }
@@ -412,12 +494,17 @@ int w8_status(bool reset) {
     return cudaMemcpyFromSymbol(&v, g_w8_status, sizeof(int)) == cudaSuccess ? v : SPGT_ERR_LAUNCH;
 }
 
-template <class T, bool VEC, int BN> static int w8_launch(const W8Params& p, int tiles, cudaStream_t st) {
+template <class T, int MODE, int BN> static int w8_launch(const W8Params& p, int tiles, cudaStream_t st) {
+    using W = W8<T, BN, MODE>;
     static SmemOptIn configured;
-    if (int e = smem_opt_in(weight_gradient8_kernel<T, VEC, BN>, W8<T, BN>::SMEM, configured)) return e;
+    if (int e = smem_opt_in(weight_gradient8_kernel<T, MODE, BN>, W::SMEM, configured)) return e;
     ChainScope chain;
-    if (int e = launch_chained(weight_gradient8_kernel<T, VEC, BN>, dim3((unsigned)p.splits, (unsigned)tiles), W8_THREADS, W8<T, BN>::SMEM, st, p)) return e;
-    return launch_chained(weight_gradient8_reduce_kernel<BN>, dim3((unsigned)(tiles * (W8_T * BN / 4 / 32) + (p.db ? tiles / p.kt * (W8_T / 32) : 0))), 256, 0, st, p, tiles);
+    if (int e = launch_chained(weight_gradient8_kernel<T, MODE, BN>, dim3((unsigned)p.splits, (unsigned)tiles), W::THREADS, W::SMEM, st, p)) return e;
+    return launch_chained(weight_gradient8_reduce_kernel<BN>, dim3((unsigned)(tiles * (W8_T * BN / 4 / 32) + (p.db ? tiles / p.kt * (W8_T / 32) : 0))), 32 * W8_SHARES, 0, st, p, tiles);
+}
+template <class T, int BN> static int w8_launch(const W8Params& p, int tiles, cudaStream_t st) {
+    if (p.N % 8 || p.K % 8) return w8_launch<T, W8_ANY, BN>(p, tiles, st);
+    return tiles == 1 && p.K % 16 == 0 && aligned16(p.steps) ? w8_launch<T, W8_WHOLE, BN>(p, tiles, st) : w8_launch<T, W8_VEC, BN>(p, tiles, st);
 }
 
 }  // namespace spgt
@@ -442,8 +529,6 @@ extern "C" int spgt_weight_gradient8(const void* dy, int dtype, const int8_t* co
     p.colpart = p.partial + (size_t)p.splits * tiles * W8_T * width;
     return with_type(dtype, [&](auto zero) {
         using T = decltype(zero);
-        const bool vec = N % 8 == 0 && K % 8 == 0;
-        if (width == W8_T) return vec ? w8_launch<T, true, W8_T>(p, tiles, (cudaStream_t)stream) : w8_launch<T, false, W8_T>(p, tiles, (cudaStream_t)stream);
-        return vec ? w8_launch<T, true, 2 * W8_T>(p, tiles, (cudaStream_t)stream) : w8_launch<T, false, 2 * W8_T>(p, tiles, (cudaStream_t)stream);
+        return width == W8_T ? w8_launch<T, W8_T>(p, tiles, (cudaStream_t)stream) : w8_launch<T, 2 * W8_T>(p, tiles, (cudaStream_t)stream);
     });
 }

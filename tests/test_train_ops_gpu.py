@@ -368,6 +368,32 @@ def test_weight_gradient8(dtype, rows, N, K):
     assert torch.equal(again[0], dw) and again[1] is None
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows', [1, 31, 33, 63, 65, 129, 4765, 28421])
+@pytest.mark.parametrize('N,K', [(8, 16), (128, 112), (40, 128), (128, 144), (120, 240), (128, 256)])
+def test_weight_gradient8_one_tile(dtype, rows, N, K):
+    """Widths of one tile, whose blocks are copied as they lie in memory where the steps start on a 16-byte boundary and piece by piece where
+    they do not: the same result, and rows past the end count for nothing."""
+    from spgt_b200 import ops
+    x, dy = _rand(rows, K, seed=1, dtype=dtype, mean=0.5), _rand(rows, N, seed=2, dtype=dtype)
+    kept = ops.compress8(x)
+    dw, db = ops.weight_gradient8(dy, kept)
+    v, d = _kept64(x), dy.double()
+    _within(dw, d.t() @ v, 192 * U * (d.abs().t() @ v.abs()) + 1e-37)
+    _within(db, d.sum(0), (192 + rows / 2000) * U * d.abs().sum(0))
+    room = torch.empty(kept.steps.numel() + 1, device='cuda', dtype=torch.uint8)
+    room[1:] = kept.steps
+    dw1, db1 = ops.weight_gradient8(dy, ops.Checkpoint8(kept.codes, room[1:], x.shape, dtype))
+    assert torch.equal(dw, dw1) and torch.equal(db, db1)
+    # what lies behind the last row is not read into the sums
+    more = torch.full((rows + 64, N), float('nan'), device='cuda', dtype=dtype)
+    more[:rows] = dy
+    codes = torch.cat((kept.codes.view(-1), torch.full((64 * K,), 127, device='cuda', dtype=torch.int8)))
+    steps = torch.cat((kept.steps.view(-1), torch.full((64 * K // 32 + 1,), 255, device='cuda', dtype=torch.uint8)))
+    dw2, db2 = ops.weight_gradient8(more[:rows], ops.Checkpoint8(codes[:rows * K], steps[:(rows * K + 31) // 32], x.shape, dtype))
+    assert torch.equal(dw, dw2) and torch.equal(db, db2)
+
+
 def test_weight_gradient8_no_rows():
     from spgt_b200 import ops
     dw, db = ops.weight_gradient8(torch.empty(0, 5, device='cuda'), ops.compress8(torch.empty(0, 9, device='cuda')))
