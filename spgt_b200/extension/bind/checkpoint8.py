@@ -53,7 +53,9 @@ def activation8(X: Tensor, activation) -> Tensor:
 
 
 def linear8(X: Tensor, weight: Tensor, bias: Tensor = None) -> Tensor:
-    """X weight^T + bias (torch's linear), of which the backward pass keeps X in 8 bits."""
+    """X weight^T + bias (torch's linear), of which the backward pass keeps X in 8 bits; up to ops.WEIGHT8_MOST features in and out."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (X, weight, bias)):
+        if max(weight.shape) > ops.WEIGHT8_MOST:            # (not first in the backward pass)
+            raise ValueError(f'linear8 takes up to {ops.WEIGHT8_MOST} features, got {tuple(weight.shape)}')
         return Linear8_Function.apply(X, weight, bias)
     return torch.nn.functional.linear(X, weight, bias)

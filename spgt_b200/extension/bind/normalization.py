@@ -34,4 +34,4 @@ def group_norm_act(X: Tensor, num_groups: int, weight: Tensor = None, bias: Tens
         raise ValueError('activation_bits must be 8 or 32')
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (X, weight, bias)):
         return Group_Norm_Act_Function.apply(X, weight, bias, num_groups, eps, activation, activation_bits)
-    return ops.group_norm_forward(X, num_groups, weight, bias, eps, activation, False)[0]
+    return ops.group_norm_forward(X.contiguous(), num_groups, weight, bias, eps, activation, False)[0]

@@ -560,3 +560,53 @@ def test_refusals_on_device():
         g, = torch.autograd.grad(f(t).square().sum(), t, create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum(), t)
+
+
+def test_calls_with_and_without_gradients_agree():
+    """The same arguments are taken, and refused, whether or not a gradient is wanted."""
+    from spgt_b200 import ops
+    from spgt_b200.extension.bind.checkpoint8 import activation8, linear8
+    from spgt_b200.extension.bind.normalization import group_norm_act
+    x = _rand(2, 24, 9, 8, seed=1).permute(0, 2, 3, 1)          # not contiguous
+    for f in (lambda t: group_norm_act(t, 4, None, None, 1e-5, 'silu'), lambda t: activation8(t, 'silu'),
+              lambda t: linear8(t, torch.ones(3, 24, device='cuda'))):
+        with torch.no_grad():
+            want = f(x)
+        assert torch.equal(f(x.clone(memory_format=torch.preserve_format).requires_grad_()).detach(), want)
+        assert torch.equal(f(x.contiguous()), want)
+    wide = ops.WEIGHT8_MOST + 1
+    for w in (torch.ones(2, wide, device='cuda'), torch.ones(wide, 2, device='cuda')):
+        with pytest.raises(ValueError):                         # before anything is kept for a backward pass that could not run
+            linear8(torch.ones(3, w.shape[1], device='cuda', requires_grad=True), w)
+
+
+def test_weight_gradient8_widest():
+    from spgt_b200 import ops
+    for N, K in ((ops.WEIGHT8_MOST, 40), (40, ops.WEIGHT8_MOST), (ops.WEIGHT8_MOST - 3, 33)):
+        x, dy = _rand(67, K, seed=1), _rand(67, N, seed=2)
+        kept = ops.compress8(x)
+        dw, db = ops.weight_gradient8(dy, kept)
+        v, d = _kept64(x), dy.double()
+        _within(dw, d.t() @ v, 192 * U * (d.abs().t() @ v.abs()) + 1e-37)
+        _within(db, d.sum(0), 192 * U * d.abs().sum(0))
+
+
+@pytest.mark.parametrize('N,P,C,G', [(3000, 4, 8, 2), (1, 1, 2048, 64), (300, 1, 250, 5), (7, 2, 3, 3)])
+def test_group_norm_backward_many_rows_of_sums(N, P, C, G):
+    """Parameter gradients over many small samples and few or many channels."""
+    from spgt_b200 import ops
+    x, dy, w, b = _rand(N, P, C, seed=1), _rand(N, P, C, seed=2), _rand(C, seed=3), _rand(C, seed=4)
+    y, stats, _ = ops.group_norm(x, G, w, b, 1e-3, None)
+    dx, dw, db = ops.group_norm_backward(dy, x, G, w, b, stats, None)
+    d, m, r = dy.double(), stats[..., 0].double(), stats[..., 1].double()
+    xh = (x.double().view(N, P, G, -1) - m[:, None, :, None]) * r[:, None, :, None]
+    xh = xh.reshape(N, P, C)
+    # a sum of N P terms in chains of at most N / 128 + 64 + 12 additions, each term with the few roundings of xh
+    n = N * P // 64 + 100
+    _within(db, d.sum((0, 1)), n * U * d.abs().sum((0, 1)) + 1e-30)
+    _within(dw, (d * xh).sum((0, 1)), n * U * (d * xh).abs().sum((0, 1)) + 1e-30)
+    wd = (w.double() * d).view(N, P, G, -1)
+    xg = xh.view(N, P, G, -1)
+    want = r[:, None, :, None] * (wd - wd.mean((1, 3), keepdim=True) - xg * (wd * xg).mean((1, 3), keepdim=True))
+    size = r[:, None, :, None] * (wd.abs() + wd.abs().mean((1, 3), keepdim=True) + xg.abs() * (wd * xg).abs().mean((1, 3), keepdim=True))
+    _within(dx.view(N, P, G, -1), want, 100 * U * size + 1e-30)
