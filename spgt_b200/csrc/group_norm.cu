@@ -15,12 +15,13 @@
 // sample's words themselves.  Both read x, so they take turns over units of samples that stay in L2 in between: the first pass asks L2
 // to keep what it reads, the second to let go of what it reads and writes.  Launches are chained (common.cuh), which hides their gaps.
 // Measured, in a graph, with what reading x (and dy) and writing the result once takes at the measured copy rate: 64 x 106 x 106 x 128
-// fp32 174 us (112; part of the second read comes from memory, and a unit's passes each start and drain), 8 x 211 x 211 x 42 bf16 24.5
-// (9.1; two waves' latencies), 43 x 43 x 128 fp32 7.7 (0.3; two launches); backward of 4 x 71 x 71 x 128 fp32 15.9 (4.7), of 16 x 106 x
-// 106 x 128 fp32 from a checkpoint 64 (32), of 8 x 211 x 211 x 44 bf16 from one 36.3 (12).
+// fp32 172 us (112; part of the second read comes from memory, and a unit's passes each start and drain), 8 x 211 x 211 x 42 bf16 23.7
+// (9.1; two waves' latencies), 43 x 43 x 128 fp32 7.3 (0.3; two launches); backward of 4 x 71 x 71 x 128 fp32 15.9 (4.7), of 16 x 106 x
+// 106 x 128 fp32 from a checkpoint 64 (32), of 8 x 211 x 211 x 44 bf16 from one 35.4 (12).
 // One launch in which a cluster of 8 or 16 blocks shares a sample and meets in the middle is no faster: 178 to 191 us, 37 and 9.5 for
 // the first three.
 #include "lowp.cuh"
+#include <type_traits>
 
 namespace spgt {
 
@@ -145,6 +146,42 @@ template <int U, int B, class L, class F> __device__ __forceinline__ void gn_vec
         }
     }
 }
+// The same in two parts, so that the first batches can be under way before what f needs.
+template <int U, int B, class L> struct GnStream {
+    using Loaded = std::invoke_result_t<L, int>;
+    const L load;
+    const int mine, period, left, last;
+    Loaded r[B][U];
+    __device__ __forceinline__ GnStream(const GnTask& t, const GnThread& me, L l)
+        : load(l), mine(me.mine), period(me.period), left(me.active ? t.left : 0), last(t.left - 1 - (t.left - 1 - me.mine) % me.period) {}
+    __device__ __forceinline__ void fetch(Loaded (&to)[U], int j) {
+        if (j >= left) return;
+#pragma unroll
+        for (int u = 0; u < U; ++u) to[u] = load(min(j + u * period, last));
+    }
+    __device__ __forceinline__ void start() {
+#pragma unroll
+        for (int b = 0; b < B; ++b) fetch(r[b], mine + b * U * period);
+    }
+    template <class F> __device__ __forceinline__ void run(F&& f) {
+        for (int j = mine; j < left; j += B * U * period) {
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int jb = j + b * U * period;
+                if (jb < left) {
+                    f(jb, r[b]);
+                    fetch(r[b], jb + B * U * period);
+                }
+            }
+        }
+    }
+};
+template <int U, int B, class L> __device__ __forceinline__ GnStream<U, B, L> gn_stream(const GnTask& t, const GnThread& me, L load) { return GnStream<U, B, L>(t, me, load); }
+// Whether a second pass loads its first batches before it waits for the sums (no kernel of the chain writes what it loads): 16-bit types,
+// whose blocks are few (8 x 211 x 211 x 42 bf16 24.6 -> 23.7 us, 64 x 106 x 106 x 128 bf16 112.8 -> 108.9, backward 188 -> 183).  fp32 loads them
+// after that, forward next to the parameters (64 x 106 x 106 x 128 175 -> 172; before the wait 186); backward all in one place: in two parts
+// the compiler's code is slower (16 x 106 x 106 x 128 from a checkpoint 64 -> 80).
+template <int V> constexpr bool GN_EARLY = V == 8;
 template <class F> __device__ __forceinline__ void gn_with_act(int act, F&& f) {
     if (act == SPGT_ACT_SILU) f(std::integral_constant<int, SPGT_ACT_SILU>{});
     else if (act == SPGT_ACT_RELU) f(std::integral_constant<int, SPGT_ACT_RELU>{});
@@ -345,12 +382,15 @@ template <class T, bool JOINT, bool KEEP> __global__ void __launch_bounds__(GN_M
     const GnTask t = gn_task<V>(s, p.first + n_in, s.tiles - 1 - (int)(blockIdx.x - n_in * s.tiles));
     const GnThread me(s);
     const uint64_t drop = gn_drop();
+    const T* x = (const T*)p.x + t.base;
+    auto vectors = gn_stream<U, V == 4 ? 1 : 2>(t, me, [&](int j) { return gn_raw(x + (int64_t)j * V, drop); });
+    if constexpr (GN_EARLY<V>) vectors.start();
     pdl_wait();
     gn_groups(s, s_group, [&](int g) { return gn_merge_stats(p, t, g); });
+    if constexpr (!GN_EARLY<V>) vectors.start();
     if (t.tile == 0)
         for (int g = threadIdx.x; g < s.G; g += s.work) p.stats[(int64_t)t.n * s.G + g] = s_group[g];
     const GnChannels<V, JOINT> ch(p, t, me, [&](int g) { return s_group[g]; });
-    const T* x = (const T*)p.x + t.base;
     gn_with_act(p.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
         if (threadIdx.x < t.head_here + t.tail_here) {
@@ -361,7 +401,7 @@ template <class T, bool JOINT, bool KEEP> __global__ void __launch_bounds__(GN_M
             act_values(ACT, z);
             ((T*)p.out)[t.first + at] = from_f32<T>(z[0]);
         }
-        gn_vectors<U, V == 4 ? 1 : 2>(t, me, [&](int j) { return gn_raw(x + (int64_t)j * V, drop); }, [&](int j0, const uint4 (&batch)[U]) {
+        vectors.run([&](int j0, const uint4 (&batch)[U]) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int j = j0 + u * me.period;
@@ -564,6 +604,9 @@ template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_
     const GnThread me(s);
     const float2* stats = p.stats + (int64_t)t.n * s.G;
     const uint64_t drop = gn_drop();
+    auto load = [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, drop); };
+    auto vectors = gn_stream<U, GN_BWD_AHEAD<V>>(t, me, load);
+    if constexpr (GN_EARLY<V>) vectors.start();
     pdl_wait();
     gn_groups(s, s_group, [&](int g) { return gn_bwd_merge(p, t, g); });
     const GnChannels<V, JOINT> ch(p, t, me, [&](int g) { return stats[g]; });
@@ -591,7 +634,7 @@ template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_
             act_slopes(ACT, z, d);
             ((T*)p.out)[t.first + at] = from_f32<T>(fmaf(xm, -st.y * st.y * k.y, fmaf(a, d[0], -st.y * k.x)));
         }
-        gn_vectors<U, GN_BWD_AHEAD<V>>(t, me, [&](int j) { return gn_load_pair<T, CODES>(p, t.base + (int64_t)j * V, drop); }, [&](int j0, const GnPair<V, CODES> (&batch)[U]) {
+        auto use = [&](int j0, const GnPair<V, CODES> (&batch)[U]) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int j = j0 + u * me.period;
@@ -606,7 +649,9 @@ template <class T, bool JOINT, bool CODES> __global__ void __launch_bounds__(GN_
                 }
                 __stcs(reinterpret_cast<uint4*>((T*)p.out + t.base + (int64_t)j * V), pack_pairs(d, T{}));
             }
-        });
+        };
+        if constexpr (GN_EARLY<V>) vectors.run(use);
+        else gn_vectors<U, GN_BWD_AHEAD<V>>(t, me, load, use);
     });
     if (p.last) gn_params(p, s_group);
 }
