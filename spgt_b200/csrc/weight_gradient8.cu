@@ -11,7 +11,7 @@
 // for 179776, a plain fp32 product's 5e-7 and 1.3e-6.
 // Blocks split the rows; their results are added by a second kernel in order.
 // Bound by what the loading warps do: of 179776 rows, dy 128 columns and x 256 in fp32, 42 us, about 10 are the start, the blocks' partial
-// results and their sum; the copies alone take 22 (118 MB, at the measured rate 18), conversion alone about as long (a block of 32 rows,
+// results and their sum; the copies alone take 22 (140 MB, at the measured copy rate 21), conversion alone about as long (a block of 32 rows,
 // of which a multiprocessor has 38, is split, stored and multiplied in some 0.8 us), and the two overlap in part.  fp16 36 us, bf16 33; dy 256
 // columns, x 128: fp32 59; dy 130, x 250: fp32 165; 7396 rows, 128 x 136 bf16: 11.
 //   Warps 0-15 load and convert, 16-19 write the results, the first of those issues the MMAs, and 20 copies where blocks are runs of
