@@ -438,7 +438,7 @@ int spgt_weight_gradient8(const void* dy, int dtype, const int8_t* codes, const 
                           int64_t rows, void* workspace, size_t workspace_bytes, spgt_stream_t stream);
 
 /* y = act((x - m) / sqrt(v + eps) * w + b) for x, y [N, P, C] with mean m and biased variance v of each sample's and group's P * C / G
- * values; w, b [C] or NULL (1, 0).  stats [N, G, 2] receives m and 1 / sqrt(v + eps).  With codes and steps a checkpoint of x is
+ * values; w, b [C] or NULL (1, 0).  stats [N, G, 2] receives m and 1 / sqrt(v + eps), zeros where P is 0.  With codes and steps a checkpoint of x is
  * written as well.  G divides C; C is up to 512, or up to 2048 (fp32) and 4096 (bf16, fp16) in multiples of 16 bytes.
  * 0 bytes: unsupported sizes.  y may be x unless a checkpoint is written. */
 size_t spgt_group_norm_workspace_bytes(int N, int64_t P, int C, int G, int dtype);

@@ -722,12 +722,15 @@ extern "C" int spgt_group_norm_fwd(const void* x, const float* w, const float* b
     GnParams p{};
     if (int e = gn_shape(N, P, C, G, dtype, 1, false, p.s)) return e;
     if (act < SPGT_ACT_NONE || act > SPGT_ACT_SILU2) return SPGT_ERR_SHAPE;
-    if (N == 0 || P == 0) return SPGT_OK;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (N == 0 || P == 0) {                                 // no pixels: the statistics are zero
+        if (N > 0 && stats && cudaMemsetAsync(stats, 0, (size_t)N * G * sizeof(float2), st) != cudaSuccess) return launch_status();
+        return SPGT_OK;
+    }
     if (!x || !y || !stats || !workspace || !codes != !steps) return SPGT_ERR_NULL;
     if (workspace_bytes < spgt_group_norm_workspace_bytes(N, P, C, G, dtype)) return SPGT_ERR_WORKSPACE;
     if (!aligned16(x) || !aligned16(y) || !aligned16(stats) || !aligned16(workspace) || (codes && !aligned16(codes))) return SPGT_ERR_ALIGN;
     const GnShape& s = p.s;
-    const cudaStream_t st = (cudaStream_t)stream;
     p.words = (float2*)workspace;
     p.x = x; p.out = y; p.w = w; p.b = b; p.stats = (float2*)stats; p.eps = eps; p.act = act;
     p.out_codes = codes; p.out_steps = steps;

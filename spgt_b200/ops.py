@@ -982,7 +982,7 @@ def group_norm_forward(x: Tensor, num_groups: int, weight: Optional[Tensor], bia
 def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1.0e-5, act=None,
                compress: bool = False):
     """(act(group_norm(x) * weight + bias), statistics [N, num_groups, 2], x in 8 bits or None) for x [N, ..., C], channels last;
-    weight, bias [C] fp32 or None.  The statistics: mean and 1 / sqrt(variance + eps)."""
+    weight, bias [C] fp32 or None.  The statistics: mean and 1 / sqrt(variance + eps), zeros where there are no pixels."""
     y, buf, kept = group_norm_forward(x, num_groups, weight, bias, eps, act, compress)
     return y, buf[:2 * x.shape[0] * num_groups].view(x.shape[0], num_groups, 2), kept
 
