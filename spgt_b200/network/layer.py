@@ -172,7 +172,8 @@ class ConvResBlock2D(_KernelWeights):
         self.activation = activation
         self.conv_layer = torch.nn.Conv2d(in_dim, out_dim, kernel_size=kernel_size, padding=padding)
         if num_group > 0:
-            self.norm_layer = GroupNormAct(max(g for g in range(1, min(num_group, out_dim) + 1) if out_dim % g == 0), out_dim, activation)
+            self.norm_layer = GroupNormAct(max(g for g in range(1, min(num_group, out_dim) + 1) if out_dim % g == 0), out_dim,
+                                           activation if activation in ops.ACT else 'relu')
 
     @property
     def norm(self):
@@ -253,6 +254,6 @@ class FeedForward(_KernelWeights):
     def forward_train(self, X: Tensor) -> Tensor:
         if self.activation_bits == 8 and plain_linears(self._watch, self, self.layer1, self.layer2):
             from ..extension.bind.checkpoint8 import activation8, linear8
-            H = activation8(linear8(X, self.layer1.weight, self.layer1.bias), self.activation)
+            H = activation8(linear8(X, self.layer1.weight, self.layer1.bias), 'silu' if self.activation == 'silu' else 'relu')
             return linear8(H, self.layer2.weight, self.layer2.bias)
         return self.layer2(_act(self.activation)(self.layer1(X)))

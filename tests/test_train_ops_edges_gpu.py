@@ -15,3 +15,21 @@ def test_statistics_of_no_pixels_are_zero():
         del dirt
         y, stats, _ = ops.group_norm(torch.empty(shape, device='cuda'), 3, None, None)
         assert y.shape == shape and stats.shape == (shape[0], 3, 2) and torch.equal(stats, torch.zeros_like(stats))
+
+
+def test_layers_follow_the_rule_of_the_configuration():
+    """The model's layers take 'silu' as SiLU and any other name as ReLU, with the options as without."""
+    from spgt_b200.network.layer import ConvResBlock2D, FeedForward
+    torch.manual_seed(0)
+    x = _rand(5, 40, seed=1).requires_grad_()
+    image = _rand(2, 6, 9, 11, seed=2)
+    for name in ('gelu', 'none', 'silu2', 'relu', 'silu'):
+        ffn = FeedForward(40, 40, 64, 0.0, name).cuda()
+        want = ffn.forward_train(x)
+        ffn.activation_bits = 8
+        assert rel_l2(ffn.forward_train(x), want) < 1e-5
+    block = ConvResBlock2D(6, 24, 3, 1, 0.0, 'gelu', num_group=4).cuda()
+    with torch.backends.cudnn.flags(allow_tf32=False):
+        z = block.conv_layer(image)
+        want = torch.relu(torch.nn.functional.group_norm(z, 4, block.norm.weight, block.norm.bias, 1e-5))
+        assert rel_l2(block.forward_train(image), want) < 1e-5
