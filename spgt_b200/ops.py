@@ -25,6 +25,15 @@ def act_code(name) -> int:
     return 1
 
 
+def _act_known(name) -> int:
+    """The code of an activation that the training operators know.  They have no configuration of the reference to follow, so any
+    other name is an error."""
+    code = ACT.get(name)
+    if code is None:
+        raise ValueError(f'activation must be one of {", ".join(map(repr, ACT))}, got {name!r}')
+    return code
+
+
 def _stream() -> int:
     """The current stream's handle, without the Stream object that torch.cuda.current_stream() makes (5 us of a small call)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
@@ -884,7 +893,7 @@ def activation8(x: Tensor, act) -> Tuple[Tensor, Checkpoint8]:
     x = _aligned(x)
     with _device(x.device):
         kept, y = Checkpoint8._empty(x), torch.empty_like(x)
-        _call('spgt_compress8', x.data_ptr(), code, act_code(act), y.data_ptr(), kept.codes.data_ptr(), kept.steps.data_ptr(), x.numel(), _stream())
+        _call('spgt_compress8', x.data_ptr(), code, _act_known(act), y.data_ptr(), kept.codes.data_ptr(), kept.steps.data_ptr(), x.numel(), _stream())
     return y, kept
 
 
@@ -894,7 +903,7 @@ def activation8_backward(grad_out: Tensor, kept: Checkpoint8, act) -> Tensor:
     grad_out = _aligned(_same(grad_out, 'grad_out', kept.shape, kept.codes.device))
     with _device(grad_out.device):
         dx = torch.empty_like(grad_out)
-        _call('spgt_restore8', kept.codes.data_ptr(), kept.steps.data_ptr(), grad_out.data_ptr(), act_code(act), dx.data_ptr(), code, dx.numel(), _stream())
+        _call('spgt_restore8', kept.codes.data_ptr(), kept.steps.data_ptr(), grad_out.data_ptr(), _act_known(act), dx.data_ptr(), code, dx.numel(), _stream())
     return dx
 
 
@@ -974,7 +983,7 @@ def group_norm_forward(x: Tensor, num_groups: int, weight: Optional[Tensor], bia
             kept = Checkpoint8._empty(x)
             codes, steps = kept.codes.data_ptr(), kept.steps.data_ptr()
         stats = buf.data_ptr()
-        _call('spgt_group_norm_fwd', x.data_ptr(), w, b, y.data_ptr(), stats, codes, steps, N, P, C, num_groups, eps, act_code(act), code, stats + stats_bytes, need,
+        _call('spgt_group_norm_fwd', x.data_ptr(), w, b, y.data_ptr(), stats, codes, steps, N, P, C, num_groups, eps, _act_known(act), code, stats + stats_bytes, need,
               _stream(), kernels=_norm_launches(N, P * C * x.element_size()) + (compress and C % 32 != 0 and N * P > 0))
     return y, buf, kept
 
@@ -1013,6 +1022,6 @@ def group_norm_backward(grad_out: Tensor, x, num_groups: int, weight: Optional[T
         dw, db = grad_out.new_empty(C, dtype=torch.float32), grad_out.new_empty(C, dtype=torch.float32)
         ws = grad_out.new_empty(need, dtype=torch.uint8)
         _call('spgt_group_norm_bwd', grad_out.data_ptr(), values, codes, steps, w, b, stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
-              N, P, C, num_groups, act_code(act), code, ws.data_ptr(), need, _stream(),
+              N, P, C, num_groups, _act_known(act), code, ws.data_ptr(), need, _stream(),
               kernels=_norm_launches(N, P * C * dx.element_size() * 2 if codes is None else P * C * (dx.element_size() + 1)))
     return dx, dw, db

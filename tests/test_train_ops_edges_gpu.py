@@ -17,6 +17,24 @@ def test_statistics_of_no_pixels_are_zero():
         assert y.shape == shape and stats.shape == (shape[0], 3, 2) and torch.equal(stats, torch.zeros_like(stats))
 
 
+def test_unknown_activations_are_refused():
+    """A name that the operators do not know is an error, with and without gradients, and not another activation."""
+    from spgt_b200 import ops
+    from spgt_b200.extension.bind.checkpoint8 import activation8
+    from spgt_b200.extension.bind.normalization import group_norm_act
+    x = _rand(2, 4, 4, 12, seed=1)
+    leaf = x.clone().requires_grad_()
+    kept = ops.compress8(x)
+    stats = ops.group_norm(x, 3, None, None)[1]
+    for name in ('gelu', 'tanh', 'ReLU', ''):
+        for call in (lambda: group_norm_act(x, 3, activation=name), lambda: group_norm_act(leaf, 3, activation=name), lambda: activation8(x, name),
+                     lambda: activation8(leaf, name), lambda: ops.group_norm(x, 3, None, None, act=name),
+                     lambda: ops.group_norm_backward(x, x, 3, None, None, stats, name), lambda: ops.activation8(x, name),
+                     lambda: ops.activation8_backward(x, kept, name)):
+            with pytest.raises(ValueError, match='activation'):
+                call()
+
+
 def test_layers_follow_the_rule_of_the_configuration():
     """The model's layers take 'silu' as SiLU and any other name as ReLU, with the options as without."""
     from spgt_b200.network.layer import ConvResBlock2D, FeedForward
