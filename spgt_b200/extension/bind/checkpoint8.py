@@ -26,21 +26,24 @@ class Activation8_Function(torch.autograd.Function):
 class Linear8_Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, X, weight, bias):
-        kept = ops.compress8(X.contiguous())
         ctx.args = (X.shape, X.dtype, bias is not None)
-        ctx.save_for_backward(weight, kept.codes, kept.steps)
+        if any(ctx.needs_input_grad[1:]):
+            kept = ops.compress8(X.contiguous())
+            ctx.save_for_backward(weight, kept.codes, kept.steps)
+        else:                                               # a frozen layer
+            ctx.save_for_backward(weight)
         return torch.nn.functional.linear(X, weight, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        weight, codes, steps = ctx.saved_tensors
+        weight, *kept = ctx.saved_tensors
         shape, dtype, has_bias = ctx.args
         dX = dw = db = None
         if ctx.needs_input_grad[0]:
             dX = torch.matmul(grad_out, weight.to(grad_out.dtype)).to(dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw, db = ops.weight_gradient8(grad_out.contiguous(), ops.Checkpoint8._of(codes, steps, shape, dtype), column_sums=has_bias)
+            dw, db = ops.weight_gradient8(grad_out.contiguous(), ops.Checkpoint8._of(*kept, shape, dtype), column_sums=has_bias)
             dw, db = dw.to(weight.dtype), None if db is None else db.to(weight.dtype)
         return dX, dw, db
 
@@ -53,7 +56,8 @@ def activation8(X: Tensor, activation) -> Tensor:
 
 
 def linear8(X: Tensor, weight: Tensor, bias: Tensor = None) -> Tensor:
-    """X weight^T + bias (torch's linear), of which the backward pass keeps X in 8 bits; up to ops.WEIGHT8_MOST features in and out."""
+    """X weight^T + bias (torch's linear), of which the backward pass keeps X in 8 bits (nothing of X where weight and bias are
+    frozen); up to ops.WEIGHT8_MOST features in and out."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (X, weight, bias)):
         if max(weight.shape) > ops.WEIGHT8_MOST:            # (not first in the backward pass)
             raise ValueError(f'linear8 takes up to {ops.WEIGHT8_MOST} features, got {tuple(weight.shape)}')

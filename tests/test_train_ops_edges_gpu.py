@@ -51,3 +51,22 @@ def test_layers_follow_the_rule_of_the_configuration():
         z = block.conv_layer(image)
         want = torch.relu(torch.nn.functional.group_norm(z, 4, block.norm.weight, block.norm.bias, 1e-5))
         assert rel_l2(block.forward_train(image), want) < 1e-5
+
+
+def test_frozen_layer_keeps_no_checkpoint():
+    from spgt_b200.extension.bind.checkpoint8 import linear8
+    x, w, b = _rand(4096, 64, seed=1).requires_grad_(), _rand(32, 64, seed=2), _rand(32, seed=3)
+    dy = _rand(4096, 32, seed=4)
+    linear8(x, w, b)                                            # (the library's workspace is allocated once)
+    before = torch.cuda.memory_allocated()
+    y = linear8(x, w, b)
+    assert torch.cuda.memory_allocated() - before == y.numel() * 4
+    dx, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(dx, dy @ w)
+    # only the bias, or only the weight
+    lw, lb = w.clone().requires_grad_(), b.clone().requires_grad_()
+    want_w, want_b = torch.autograd.grad(linear8(x.detach(), lw, lb), (lw, lb), dy)
+    got, = torch.autograd.grad(linear8(x.detach(), w, lb), lb, dy)
+    assert torch.equal(got, want_b)
+    got, = torch.autograd.grad(linear8(x.detach(), lw, b), lw, dy)
+    assert torch.equal(got, want_w)
