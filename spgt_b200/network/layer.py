@@ -221,9 +221,10 @@ def _act(name):
 
 
 def plain_linears(watch: ParameterWatch, module: torch.nn.Module, *linears) -> bool:
-    """Whether calls of the module's linear layers may be replaced by operators on their parameters: layers of torch's own type that
-    nothing watches, on the GPU."""
-    return (all(type(l) is torch.nn.Linear and l.weight.is_cuda for l in linears)
+    """Whether calls of the module's linear layers may be replaced by linear8: layers of torch's own type that nothing watches, on the
+    GPU, of types and widths that it takes."""
+    return (all(type(l) is torch.nn.Linear and l.weight.is_cuda and l.weight.dtype in ops.DTYPE
+                and 0 < min(l.weight.shape) and max(l.weight.shape) <= ops.WEIGHT8_MOST for l in linears)
             and not watch.observed(module) and not watch.backward_observed(*linears))
 
 

@@ -70,3 +70,19 @@ def test_frozen_layer_keeps_no_checkpoint():
     assert torch.equal(got, want_b)
     got, = torch.autograd.grad(linear8(x.detach(), lw, b), lw, dy)
     assert torch.equal(got, want_w)
+
+
+@pytest.mark.parametrize('dims,dtype', [((8, 4100, 16), torch.float32), ((4100, 8, 16), torch.float32), ((8, 8, 4100), torch.float32), ((12, 20, 30), torch.float64)])
+def test_feed_forward_that_linear8_does_not_take(dims, dtype):
+    """Widths and types beyond linear8 train on the plain layers, as without the option."""
+    from spgt_b200.network.layer import FeedForward
+    torch.manual_seed(0)
+    ffn = FeedForward(*dims, 0.0, 'silu').cuda().to(dtype)
+    x, dy = _rand(6, dims[0], seed=1).to(dtype).requires_grad_(), _rand(6, dims[1], seed=2).to(dtype)
+
+    def step():
+        y = ffn.forward_train(x)
+        return [y.detach(), *torch.autograd.grad(y, (x, *ffn.parameters()), dy)]
+    want = step()
+    ffn.activation_bits = 8
+    assert all(torch.equal(a, c) for a, c in zip(step(), want))
