@@ -57,9 +57,9 @@ def activation8(X: Tensor, activation) -> Tensor:
 
 def linear8(X: Tensor, weight: Tensor, bias: Tensor = None) -> Tensor:
     """X weight^T + bias (torch's linear), of which the backward pass keeps X in 8 bits (nothing of X where weight and bias are
-    frozen); up to ops.WEIGHT8_MOST features in and out."""
+    frozen); 1 to ops.WEIGHT8_MOST features in and out."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (X, weight, bias)):
-        if max(weight.shape) > ops.WEIGHT8_MOST:            # (not first in the backward pass)
-            raise ValueError(f'linear8 takes up to {ops.WEIGHT8_MOST} features, got {tuple(weight.shape)}')
+        if not 0 < min(weight.shape) <= max(weight.shape) <= ops.WEIGHT8_MOST:       # (not first in the backward pass)
+            raise ValueError(f'linear8 takes 1 to {ops.WEIGHT8_MOST} features, got {tuple(weight.shape)}')
         return Linear8_Function.apply(X, weight, bias)
     return torch.nn.functional.linear(X, weight, bias)

@@ -86,3 +86,11 @@ def test_feed_forward_that_linear8_does_not_take(dims, dtype):
     want = step()
     ffn.activation_bits = 8
     assert all(torch.equal(a, c) for a, c in zip(step(), want))
+
+
+def test_linear8_without_features():
+    """A layer of no features in or out is refused before anything is kept for a backward pass that could not run."""
+    from spgt_b200.extension.bind.checkpoint8 import linear8
+    for K, N in ((0, 3), (3, 0)):
+        with pytest.raises(ValueError):
+            linear8(torch.ones(5, K, device='cuda', requires_grad=True), torch.ones(N, K, device='cuda'))
