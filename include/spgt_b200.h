@@ -431,7 +431,8 @@ int spgt_compress8(const void* x, int dtype, int act, void* y, int8_t* codes, ui
 int spgt_restore8(const int8_t* codes, const uint8_t* steps, const void* dy, int act, void* out, int dtype, int64_t n, spgt_stream_t stream);
 
 /* dw [N, K] = dy^T v and, unless NULL, db [N] = column sums of dy, for dy [rows, N] and a checkpoint of v [rows, K].
- * N and K up to 4096; products and sums as of fp32 numbers, whatever dy's type; an infinity or a NaN in dy makes its row of dw NaN.
+ * N and K up to 4096; products and sums as of fp32 numbers, whatever dy's type.  A NaN in dy makes its row of dw
+ * NaN; so does an infinity in fp32 and fp16, while in bf16 it is multiplied by the row's values of v (infinity times 0 is NaN).
  * 0 bytes: unsupported sizes. */
 size_t spgt_weight_gradient8_workspace_bytes(int N, int K, int64_t rows);
 int spgt_weight_gradient8(const void* dy, int dtype, const int8_t* codes, const uint8_t* steps, float* dw, float* db, int N, int K,

@@ -909,8 +909,8 @@ def activation8_backward(grad_out: Tensor, kept: Checkpoint8, act) -> Tensor:
 
 def weight_gradient8(grad_out: Tensor, kept: Checkpoint8, column_sums: bool = True):
     """(grad_out^T kept [N, K], column sums of grad_out [N] or None), fp32, for grad_out [..., N] and a checkpoint of [..., K]: weight and
-    bias gradient of a linear layer from its input in 8 bits.  N and K up to WEIGHT8_MOST.  A NaN or an infinity in grad_out makes its row of
-    the first NaN."""
+    bias gradient of a linear layer from its input in 8 bits.  N and K up to WEIGHT8_MOST.  A NaN in grad_out makes its row of the first
+    NaN; so does an infinity in fp32 and fp16, while in bf16 it is multiplied by its row's values of kept."""
     code = _dtype(grad_out, 'grad_out')
     if len(kept.shape) < 1 or grad_out.shape[:-1] != kept.shape[:-1] or grad_out.dim() != len(kept.shape):
         raise ValueError('grad_out must be [..., N] for a checkpoint of [..., K]')

@@ -94,3 +94,27 @@ def test_linear8_without_features():
     for K, N in ((0, 3), (3, 0)):
         with pytest.raises(ValueError):
             linear8(torch.ones(5, K, device='cuda', requires_grad=True), torch.ones(N, K, device='cuda'))
+
+
+def test_infinities_in_the_gradient():
+    """An infinity in dy: its row of dW is NaN where dy is split into parts (infinity less infinity), and in bf16 infinity times the
+    values of x; other rows are as without it."""
+    from spgt_b200 import ops
+    for dtype in TYPES:
+        x, dy = _rand(700, 64, seed=1, dtype=dtype), _rand(700, 40, seed=2, dtype=dtype)
+        x[301, 5], x[301, 6], x[301, 7] = 0.0, 2.0, -2.0
+        kept = ops.compress8(x)
+        clean, clean_db = ops.weight_gradient8(dy, kept)
+        dy[301, 9] = float('inf')
+        dy[301, 11] = float('-inf')
+        dw, db = ops.weight_gradient8(dy, kept)
+        if dtype == torch.bfloat16:
+            want = float('inf') * _kept64(x)[301]               # (zero times infinity is NaN)
+            assert want[5].isnan() and want[6] == float('inf') and want[7] == float('-inf')
+            for row, sign in ((9, 1), (11, -1)):
+                assert torch.equal(dw[row].isnan(), want.isnan()) and torch.equal(dw[row].double().nan_to_num(0, 1, -1), (sign * want).nan_to_num(0, 1, -1))
+        else:
+            assert dw[9].isnan().all() and dw[11].isnan().all()
+        rest = [i for i in range(40) if i not in (9, 11)]
+        assert torch.equal(dw[rest], clean[rest]) and torch.equal(db[rest], clean_db[rest])
+        assert db[9] == float('inf') and db[11] == float('-inf')
