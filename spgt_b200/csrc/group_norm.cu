@@ -25,7 +25,8 @@
 
 namespace spgt {
 
-constexpr int GN_MAX_WORK = 512;        // threads of a block, most
+constexpr int GN_MAX_WORK = 512;        // threads of a block, most, and vectors that they take at once: their sets, 8 bytes a value, fit 48 KB
+static_assert(GN_MAX_WORK * 8 * sizeof(float2) <= 48 * 1024, "no opt-in to more shared memory");
 
 struct GnShape {
     int64_t L;                  // values of a sample
@@ -693,9 +694,6 @@ static int gn_shape(int N, int64_t P, int C, int G, int dtype, int tensors, bool
     return SPGT_OK;
 }
 template <void (*KERNEL)(const GnParams)> static int gn_launch(GnParams p, int first, size_t smem, cudaStream_t st) {
-    static SmemOptIn configured;
-    if (smem > 48 * 1024)
-        if (int e = smem_opt_in(KERNEL, smem, configured)) return e;
     p.first = first;
     const int samples = p.s.N - first < p.s.unit ? p.s.N - first : p.s.unit;
     return launch_chained(KERNEL, dim3((unsigned)((int64_t)samples * p.s.tiles)), p.s.work, smem, st, p);
