@@ -118,3 +118,42 @@ def test_infinities_in_the_gradient():
         rest = [i for i in range(40) if i not in (9, 11)]
         assert torch.equal(dw[rest], clean[rest]) and torch.equal(db[rest], clean_db[rest])
         assert db[9] == float('inf') and db[11] == float('-inf')
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------
+# several units of samples
+# ---------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype,C,G', [(torch.bfloat16, 128, 8), (torch.bfloat16, 130, 10), (torch.float16, 130, 26), (torch.float32, 130, 10)])
+def test_group_norm_units_in_every_type(dtype, C, G):
+    """At least three units of samples either way, among them samples that start off a 16-byte boundary and checkpoints whose blocks two
+    samples share; forward out of place and in place."""
+    from spgt_b200 import ops
+    from spgt_b200._lib import lib
+    N, P = 27, 181 * 181
+    for tensors in (2, 3, 4):                                   # bytes that both passes read, in units of 96 MB
+        assert -(-N // ((96 << 20) // (P * C * tensors))) >= 3
+    x, dy = _rand(N, P, C, seed=1, mean=0.3, dtype=dtype), _rand(N, P, C, seed=2, dtype=dtype)
+    w, b = _rand(C, seed=3, mean=1.0, scale=0.2), _rand(C, seed=4)
+    y, stats, kept = ops.group_norm(x, G, w, b, 1e-5, 'silu', compress=True)
+    dx, dw, db = ops.group_norm_backward(dy, x, G, w, b, stats, 'silu')
+    dx8, dw8, db8 = ops.group_norm_backward(dy, kept, G, w, b, stats, 'silu')
+    assert torch.equal(kept.codes, ops.compress8(x).codes) and torch.equal(kept.steps, ops.compress8(x).steps)
+    x8 = _kept64(x)
+    sums = [torch.zeros(2, C, device='cuda', dtype=torch.float64) for _ in range(4)]
+    for n in range(N):
+        want = _norm64(x[n:n + 1], G, w, b, 1e-5, 'silu', dy[n:n + 1])
+        want8 = _norm64(x[n:n + 1], G, w, b, 1e-5, 'silu', dy[n:n + 1], x8[n:n + 1])
+        for got, (value, tol) in ((y, want['y']), (dx, want['dx']), (dx8, want8['dx'])):
+            _within(got[n:n + 1], value, tol + _rounded(value, dtype))
+        for s, v in zip(sums, (want['dw'], want['db'], want8['dw'], want8['db'])):
+            s += torch.stack(v)
+    # a sample's tolerance has 100 roundings of the magnitudes' sum; a thread's chain of up to 90 values, the 12 to 16 sets of a tile, and
+    # then chains of 27 * 148 / 128 tiles and 13 merges are below twice that
+    for got, (value, tol) in zip((dw, db, dw8, db8), sums):
+        _within(got, value, 2 * tol)
+    need, code = lib.spgt_group_norm_workspace_bytes(N, P, C, G, ops.DTYPE[dtype]), ops.DTYPE[dtype]
+    ws = torch.empty(need, dtype=torch.uint8, device='cuda')
+    s = torch.empty_like(stats)
+    rc = lib.spgt_group_norm_fwd(x.data_ptr(), w.data_ptr(), b.data_ptr(), x.data_ptr(), s.data_ptr(), None, None, N, P, C, G, 1e-5, 2, code,
+                                 ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(x, y) and torch.equal(s, stats)
