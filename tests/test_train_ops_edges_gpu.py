@@ -157,3 +157,25 @@ def test_group_norm_units_in_every_type(dtype, C, G):
     rc = lib.spgt_group_norm_fwd(x.data_ptr(), w.data_ptr(), b.data_ptr(), x.data_ptr(), s.data_ptr(), None, None, N, P, C, G, 1e-5, 2, code,
                                  ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
     assert rc == 0 and torch.equal(x, y) and torch.equal(s, stats)
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------
+# weight gradients of long blocks
+# ---------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,N,K', [(179776, 256, 128), (179776, 256, 512), (400000, 8, 16), (400001, 16, 240), (400000, 5, 9), (400001, 9, 130)])
+def test_weight_gradient8_many_chains(dtype, rows, N, K):
+    """Blocks of 2400 to 4900 rows: two to four times 1280, after which an accumulator's sum moves to memory and it starts again."""
+    from spgt_b200 import ops
+    splits = max(1, torch.cuda.get_device_properties(0).multi_processor_count // (-(-N // 128) * (1 if K <= 128 else -(-K // 256))))
+    assert rows / splits > 1280
+    x, dy = _rand(rows, K, seed=1, dtype=dtype, mean=0.5), _rand(rows, N, seed=2, dtype=dtype)
+    kept = ops.compress8(x)
+    dw, db = ops.weight_gradient8(dy, kept)
+    v, d = _kept64(x), dy.double()
+    # 80 additions that truncate (2 U each) before a sum moves on, at most 4 such sums, and 148 / 16 blocks' results in a row, then 15
+    _within(dw, d.t() @ v, 192 * U * (d.abs().t() @ v.abs()) + 1e-37)
+    # a thread's chain of at most rows / (16 splits) values, 32 threads, and the blocks as above
+    _within(db, d.sum(0), (rows / (16 * splits) + 64) * U * d.abs().sum(0))
+    again = ops.weight_gradient8(dy, kept)
+    assert torch.equal(again[0], dw) and torch.equal(again[1], db)
