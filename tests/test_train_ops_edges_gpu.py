@@ -179,3 +179,25 @@ def test_weight_gradient8_many_chains(dtype, rows, N, K):
     _within(db, d.sum(0), (rows / (16 * splits) + 64) * U * d.abs().sum(0))
     again = ops.weight_gradient8(dy, kept)
     assert torch.equal(again[0], dw) and torch.equal(again[1], db)
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------
+# the convolution before a normalisation
+# ---------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('bits', [32, 8])
+def test_convolution_bias_before_a_normalisation(bits):
+    """Sums of dx over a channel's pixels.  The norm takes out what a group's channels have in common, not these sums: their mean size is that of
+    dozens of pixels.  1798 pixels of dx, each off by at most 100 U of its terms, which are below 4 in the mean, and summed in fp32: below 0.06 in
+    the worst case; as independent roundings of 2 U each below 1e-4 of 30 in all, of which 1e-5 allows three times."""
+    from spgt_b200.network.layer import ConvResBlock2D
+    torch.manual_seed(0)
+    block = ConvResBlock2D(6, 42, 3, 1, 0.0, 'silu', num_group=8).cuda()
+    block.norm.activation_bits = bits
+    x = _rand(2, 6, 31, 29, seed=5).requires_grad_()
+    dy = _rand(2, 42, 31, 29, seed=6)
+    with torch.backends.cudnn.flags(allow_tf32=False, deterministic=True):
+        got, = torch.autograd.grad(block.forward_train(x), block.conv_layer.bias, dy)
+        z = block.conv_layer(x).detach().permute(0, 2, 3, 1).contiguous()
+    w, b = block.norm.weight.detach(), block.norm.bias.detach()
+    want = _norm64(z, 7, w, b, 1e-5, 'silu', dy.permute(0, 2, 3, 1).contiguous(), _kept64(z) if bits == 8 else None)['dx'][0].sum((0, 1, 2))
+    assert float(want.abs().mean()) > 10 and rel_l2(got, want) < 1e-5
