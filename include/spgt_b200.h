@@ -422,7 +422,7 @@ int spgt_darcy_forward_devbias(const spgt_darcy_model* model, const float* head_
  * A checkpoint of n values, in row-major order, is codes [n] and steps [ceil(n / 32)]: value i is codes[i] * 2^(steps[i / 32] - 127).
  * The step of 32 consecutive values is the smallest power of two (2^-126 at least) of which the largest magnitude among them is
  * less than 127.5; codes are rounded to nearest even, so a value is off by half a step at most.  A NaN or an infinity makes
- * all 32 values NaN (step 255).  Magnitudes beyond 63.5 * 2^122 become 63 * 2^122 (64 would be an infinity).
+ * all 32 values NaN (step 255).  The exception: magnitudes beyond 63.5 * 2^122 become 63 * 2^122 (64 would be an infinity).
  * ------------------------------------------------------------------------------------------- */
 
 /* codes, steps = checkpoint of x [n]; with y, also y = act(x).  y may be x. */

@@ -2,7 +2,7 @@
 // restore: the values, or a gradient times act'(values).  A thread takes 16 bytes of values at a time, so neighbouring lanes share a
 // block and every access is coalesced.  fp32: two such, loaded together, so that enough is under way (46 M values, compress 46 -> 41 us,
 // with an activation 67 -> 63; four 37 and 64, but 75 instead of 64 for its gradient); 16-bit types: one (28 us, two 29).  Bound by HBM:
-// an activation and its gradient on 46 M fp32 values take 63 + 64 us, the bytes alone 63 + 63.
+// an activation and its gradient on 46 M fp32 values take 63 + 63 us, the bytes alone 63 + 63; on bf16 40 + 39, the bytes 35 + 35.
 #include "lowp.cuh"
 
 namespace spgt {

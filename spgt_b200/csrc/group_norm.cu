@@ -12,12 +12,14 @@
 // M2 = M2a + M2b + (ma - mb)^2 na nb / (na + nb), so a mean far from zero costs no digits.  All sums have a fixed order.
 //
 // Each way is a pass for the sums, which leaves a word per group and tile, and a pass for the results, whose blocks merge their
-// sample's words themselves.  Both read x, so they take turns over units of samples that stay in L2 in between: the first pass asks L2
-// to keep what it reads, the second to let go of what it reads and writes.  Launches are chained (common.cuh), which hides their gaps.
+// sample's words themselves.  Both read x, so they take turns over units of samples that L2 could hold: the first pass asks it to keep what
+// it reads, the second to let go of what it reads and writes.  Launches are chained (common.cuh), which hides their gaps.
 // Measured, in a graph, with what reading x (and dy) and writing the result once takes at the measured copy rate: 64 x 106 x 106 x 128
-// fp32 172 us (112; part of the second read comes from memory, and a unit's passes each start and drain), 8 x 211 x 211 x 42 bf16 23.7
-// (9.1; two waves' latencies), 43 x 43 x 128 fp32 7.3 (0.3; two launches); backward of 4 x 71 x 71 x 128 fp32 15.9 (4.7), of 16 x 106 x
-// 106 x 128 fp32 from a checkpoint 64 (32), of 8 x 211 x 211 x 44 bf16 from one 35.4 (12).
+// fp32 172 us (112; reading x twice from memory would take 168, so what L2 keeps is lost again in the eight passes' starts and ends), the
+// same in bf16 109 (56), 8 x 211 x 211 x 42 bf16 23.5 (9.1; two waves' latencies), 43 x 43 x 128 fp32 7.1 (0.3; two launches), 16 x 106 x 106
+// x 128 fp32 with a checkpoint 52 (32), 8 x 211 x 211 x 44 bf16 with one, for which x is read a third time, 34 (12); backward of 4 x 71 x 71
+// x 128 fp32 15.5 (4.7), of 64 x 106 x 106 x 128 bf16 182 (84), of 16 x 106 x 106 x 128 fp32 from a checkpoint 63 (32), of 8 x 211 x 211 x 44
+// bf16 from one 35.3 (12).
 // One launch in which a cluster of 8 or 16 blocks shares a sample and meets in the middle is no faster: 178 to 191 us, 37 and 9.5 for
 // the first three.
 #include "lowp.cuh"

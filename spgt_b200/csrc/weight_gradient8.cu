@@ -10,10 +10,11 @@
 // they are added to the block's result in memory.  Error against 64 bits, relative, with normal inputs: 8.8e-8 for 7396 rows and 3.2e-7
 // for 179776, a plain fp32 product's 5e-7 and 1.3e-6.
 // Blocks split the rows; their results are added by a second kernel in order.
-// Bound by what the loading warps do: of 179776 rows, dy 128 columns and x 256 in fp32, 42 us, about 10 are the start, the blocks' partial
-// results and their sum; the copies alone take 22 (140 MB, at the measured copy rate 21), conversion alone about as long (a block of 32 rows,
-// of which a multiprocessor has 38, is split, stored and multiplied in some 0.8 us), and the two overlap in part.  fp16 36 us, bf16 33; dy 256
-// columns, x 128: fp32 59; dy 130, x 250: fp32 165; 7396 rows, 128 x 136 bf16: 11.
+// Bound by shared memory: of 179776 rows, dy 128 columns and x 256 in fp32, 42 us, about 10 are the start, the blocks' partial results and
+// their sum; in the rest a multiprocessor takes 38 blocks of 32 rows, some 0.8 us each.  For one of them 24 KB are copied in, 24 read back, 40
+// stored as parts and 72 read by the MMAs: 160 KB, 1280 cycles at 128 bytes a cycle, about 0.7 us.  (The memory's bytes take 21 us in all.)
+// fp16 35 us, bf16 32; dy 256 columns, x 128: fp32 58; 7396 rows, 128 x 136 bf16: 11, 1024 x 1024 fp32 79, bf16 65.  Widths that are no
+// multiples of eight are read value by value, nothing ahead: dy 130, x 250 fp32 165 (the bytes 21); 712336 rows, 1 x 128: 233 (15).
 //   Warps 0-15 load and convert, 16-19 write the results, the first of those issues the MMAs, and 20 copies where blocks are runs of
 // memory (W8_WHOLE).  Every wait is a bounded mbarrier poll that records a code on expiry.
 #include "lowp.cuh"
@@ -29,8 +30,8 @@ template <> struct W8Parts<__half> { static constexpr int N = 2; };
 template <> struct W8Parts<__nv_bfloat16> { static constexpr int N = 1; };
 // How the blocks of rows are read.  W8_ANY: any widths.  W8_VEC: N and K are multiples of eight, so eight columns of a row are in or out
 // together and start on a boundary of their size.  W8_WHOLE: besides, one tile holds all columns, so that a block is three runs of memory,
-// which bulk copies bring, and K is a multiple of 16 (179776 rows, 128 x 256 columns: fp32 47 us against 53, bf16 38 against 46; dy 256
-// columns, x 128 with a copy for each row of dy 113 against 64).
+// which bulk copies bring, and K is a multiple of 16 (179776 rows, 128 x 256 columns: fp32 41.5 us against 48.7 as W8_VEC, bf16 32.3 against
+// 41.8; when dy of 256 columns, x 128, took 64 us as W8_VEC, it took 113 with a copy for each row of dy).
 constexpr int W8_ANY = 0, W8_VEC = 1, W8_WHOLE = 2;
 // BN: columns of x in a tile, 128 or 256, and with it rows of a block.
 template <class T, int BN, int MODE> struct W8 {

@@ -822,8 +822,8 @@ def _aligned(t: Tensor) -> Tensor:
 
 class Checkpoint8:
     """A tensor kept in 8 bits: codes [n] (int8) and steps [ceil(n / 32)] (uint8), value i = codes[i] * 2^(steps[i // 32] - 127) in
-    row-major order; off by half a step at most, and a step is less than 1/63 of the largest magnitude among its 32 values.
-    Not finite values make their 32 values NaN."""
+    row-major order.  A value is off by half a step at most, and a step is less than 1/63 of the largest magnitude among its 32 values,
+    but not less than 2^-126; only magnitudes beyond 63.5 * 2^122 become 63 * 2^122.  Not finite values make their 32 values NaN."""
     __slots__ = ('codes', 'steps', 'shape', 'dtype')
 
     def __init__(self, codes: Tensor, steps: Tensor, shape: Sequence[int], dtype=torch.float32):
