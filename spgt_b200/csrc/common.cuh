@@ -23,8 +23,8 @@ inline int launch_status() {
 // direct predecessor has finished.  Where it comes first (group_norm.cu, weight_gradient8.cu) that does not hold while a kernel runs: before
 // its pdl_wait() such a kernel may only touch what none of the chain's earlier kernels writes, and write what none of them touches; every one
 // but a scope's first calls pdl_wait() before it ends, also where it needs nothing of the one before, so that its end still means the end of
-// all before it; and such a chain is a scope of its own, in no other.  What an earlier kernel of the chain writes is read with __ldca or cp.async, never __ldg: the
-// compiler may move a read-only load ahead of the wait.
+// all before it; and such a chain is a scope of its own, in no other.  What an earlier kernel of the chain writes is read with __ldca, __ldcg
+// or cp.async, never __ldg: the compiler may move a read-only load ahead of the wait.
 extern thread_local int g_chain;                       // 0 outside any scope, 1 before a scope's first launch, 2 after it
 struct ChainScope {
     const int before = g_chain;

@@ -124,7 +124,7 @@ class Sp_GalerkinTransformer2D(torch.nn.Module):
     config (config/darcy_config.yaml) plus 'resolution_size' and 'target_normalizer', and optionally 'num_norm_group' (group
     normalisation in the scalers' convolution blocks) and 'activation_bits' (8: training keeps the inputs of the normalisations, of
     the attention's output projections, and of the feed-forward blocks' layers and activations in 8 bits; everything else, the
-    Q, K, V projections, the convolutions and the regressor's dense and Fourier layers among it, in 32)."""
+    Q, K, V projections, the convolutions and the regressor's first and Fourier layers among it, in 32)."""
 
     def __init__(self, cfg) -> None:
         super().__init__()
